@@ -34,11 +34,22 @@ namespace kv {
 namespace {
 
 constexpr uint32_t kStepWaves = 4;
+constexpr uint32_t kJoinWaves = 8, kJoinRows = 4;  // waves on a row, or rows of a workgroup
+constexpr uint32_t kJoinFew = 16;                 // splits that one wave joins
 constexpr uint32_t kRowTile = 16;
 constexpr uint32_t kTokTile = 64;
+// Waves of a workgroup that takes all of a row tile's tokens: what the registers allow.
+constexpr uint32_t wide_waves(int d) { return d <= 192 ? 8 : 4; }
+// It needs no join, but leaves CUs idle and their bandwidth unused: up to one
+// workgroup per CU, up to so many bytes of codes for each. Measured with it and
+// with splits (and their join): 8 units of 704 tokens of 128 dimensions 10.5 and
+// 9.6 + 3.8 us, 216 units of 3500 x 64 (448 KB) 16.6 and 13.8 + 3.9 us, 128 units of 4096 x
+// 128 (1 MB) 42.5 and 31.0 + 4.1 us.
+constexpr uint64_t kWideUnits = 256, kWideBytes = 512 << 10;
 constexpr float kLift = 6.f, kSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kSplitUnits = 1024;  // workgroups that fill the chip several times over
+constexpr uint32_t kSplitTiles = 16;    // least tiles of a split: its partial sums are then 2 to 6 % of what it reads
 
 struct StepArgs {
   Cache c;
@@ -47,7 +58,7 @@ struct StepArgs {
   const int32_t* __restrict__ lists;  // LIST: tokens x kv_heads x count
   uint32_t count;
   float scale2;  // scale * log2(e)
-  uint32_t group, tiles, splits;
+  uint32_t group, tiles, outer, splits, per;  // per: tiles of 64 tokens in a split
   uint16_t* __restrict__ out;
   float* __restrict__ lse;
   float* __restrict__ part;  // splits > 1: [row][split][D] sums, then [row][split][2] (M, l)
@@ -58,23 +69,26 @@ struct Unit {
   uint32_t sq, h, tile, split;
 };
 
-template <int D, bool BF, bool LIST, bool VEC>
-__global__ __launch_bounds__(64 * kStepWaves) void k_step(StepArgs a) {
+template <int D, bool BF, bool LIST, bool VEC, uint32_t W>
+__global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
   constexpr int KS = D / 32;  // inner steps of the first product
   constexpr int DT = D / 16;  // row tiles of the second
   constexpr int KW = D / 16;  // words of a key row that a lane holds
-  __shared__ float sm_o[kStepWaves][kRowTile][D];
-  __shared__ float sm_m[kStepWaves][kRowTile], sm_l[kStepWaves][kRowTile];
+  __shared__ float sm_o[W][kRowTile][D];
+  __shared__ float sm_m[W][kRowTile], sm_l[W][kRowTile];
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const uint32_t n = lane & 15u, g = lane >> 4;
   const uint32_t bsh = a.c.bsh, bs = 1u << bsh;
   uint32_t id = blockIdx.x;
-  const uint32_t split = id % a.splits;
-  id /= a.splits;
+  // Heads fastest and splits slowest: workgroups go round the XCDs, and the first splits, which
+  // all sequences have, must not all meet on the same ones (with splits
+  // fastest, 8 of them: 215 us for a ragged batch that takes 120 like this).
   const uint32_t h = id % a.c.kvh;
   id /= a.c.kvh;
   const uint32_t tile = id % a.tiles;
   id /= a.tiles;
+  const uint32_t split = id / a.outer;
+  id %= a.outer;
   // id: the token row (LIST) or the sequence
   const uint32_t sq = LIST ? seq_at(a.b, id) : id;
   const Seq s = seq_of(a.b, sq, bsh);
@@ -100,41 +114,21 @@ __global__ __launch_bounds__(64 * kStepWaves) void k_step(StepArgs a) {
   const int32_t* const list = LIST ? a.lists + ((size_t)id * a.c.kvh + h) * a.count : nullptr;
   const int32_t* const table = a.b.table + (size_t)sq * a.b.width;
 
-  // Queries, as f16 with a power of two taken out so that bf16's range fits.
-  h8_t qf[KS];
-  float qscale = a.scale2;
-  {
-    const uint16_t* src = a.q.data + (int64_t)(s.row + tok) * a.q.token_stride + (int64_t)head * a.q.head_stride + g * (D / 4);
-    u4_t raw[KS];
-#pragma unroll
-    for (int c = 0; c < KS; ++c) {
-      if constexpr (VEC) {
-        raw[c] = *reinterpret_cast<const u4_t*>(src + 8 * c);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) raw[c][i] = (uint32_t)src[8 * c + 2 * i] | (uint32_t)src[8 * c + 2 * i + 1] << 16;
-      }
+  // this split's tiles of 64 listed tokens
+  const uint32_t all = (uint32_t)(((uint64_t)entries * bs + kTokTile - 1) / kTokTile);
+  const uint32_t t_end = split + 1 < a.splits ? min(all, (split + 1) * a.per) : all;
+  float* const part_ml = a.part + (size_t)a.b.tokens * a.q.heads * a.splits * D;  // splits > 1
+  auto row_of = [&](uint32_t rr) {
+    const uint32_t rw = r_first + rr;
+    return (size_t)(s.row + rw / a.group) * a.q.heads + h * a.group + rw % a.group;
+  };
+  if (a.splits > 1 && split * a.per >= all) {  // beyond the end
+    if (threadIdx.x < rows) {
+      float* const pm = part_ml + (row_of(threadIdx.x) * a.splits + split) * 2;
+      pm[0] = -FLT_MAX;
+      pm[1] = 0.f;
     }
-    if constexpr (BF) {
-      float mag = 0.f;
-#pragma unroll
-      for (int c = 0; c < KS; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mag = fmaxf(mag, finite_abs(load_val<true>((uint16_t)(raw[c][i >> 1] >> (16 * (i & 1))))));
-      mag = rows_max(mag);
-      int e = (int)(__float_as_uint(mag) >> 23) - 127 - 10;  // the largest becomes 2^10 .. 2^11
-      e = e < -100 ? -100 : e;
-      const float inv = exp2_int(-e);
-      qscale *= exp2_int(e);
-#pragma unroll
-      for (int c = 0; c < KS; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          qf[c][i] = (_Float16)(load_val<true>((uint16_t)(raw[c][i >> 1] >> (16 * (i & 1)))) * inv);
-    } else {
-#pragma unroll
-      for (int c = 0; c < KS; ++c) qf[c] = __builtin_bit_cast(h8_t, raw[c]);
-    }
+    return;
   }
 
   f4_t acc[DT];
@@ -142,11 +136,7 @@ __global__ __launch_bounds__(64 * kStepWaves) void k_step(StepArgs a) {
   for (int t = 0; t < DT; ++t) acc[t] = f4_t{0.f, 0.f, 0.f, 0.f};
   float M = -FLT_MAX, l = 0.f, vref = 0.f, vinv = 0.f;
 
-  // this split's tiles of 64 listed tokens
-  const uint32_t all = (uint32_t)(((uint64_t)entries * bs + kTokTile - 1) / kTokTile);
-  const uint32_t per = (all + a.splits - 1) / a.splits;
-  const uint32_t t_end = min(all, (split + 1) * per);
-  // the block with the 16 tokens of group `grp` of a tile, and its first position; a hole: -1
+  // The block with the 16 tokens of group `grp` of a tile, and its first position; a hole: -1.
   auto locate = [&](uint32_t tt, uint32_t grp, int32_t& first) -> int32_t {
     const uint32_t vt = tt * kTokTile + grp * 16u;
     const uint32_t e = vt >> bsh;
@@ -158,14 +148,26 @@ __global__ __launch_bounds__(64 * kStepWaves) void k_step(StepArgs a) {
     first = (int32_t)(((uint32_t)lg << bsh) + (vt & (bs - 1u)));
     return ph;
   };
-  for (uint32_t tt = split * per + wave; tt < t_end; tt += kStepWaves) {
-    int32_t first, other;
-    const int32_t pv = locate(tt, g, first), pk = locate(tt, n >> 2, other);
-    const uint32_t slot_v = (tt * kTokTile + g * 16u) & (bs - 1u), slot_k = (tt * kTokTile + (n >> 2) * 16u) & (bs - 1u);
-    const size_t cell_v = (size_t)max(pv, 0) * a.c.kvh + h, cell_k = (size_t)max(pk, 0) * a.c.kvh + h;
-    uint32_t kw[4][KW];
-    u4_t vw[DT];
-    const int8_t* kp = a.c.k + ((cell_k << bsh) + slot_k + (n & 3u)) * D + g * (D / 4);
+  // Loads run a tile ahead in the registers that the products have read: the
+  // next keys set out behind the first product, the next values behind the second, and
+  // the places of the tile after that one between them.
+  struct Place {
+    int32_t pk, pv, first;
+  };
+  auto place = [&](uint32_t tt) {
+    Place p;
+    int32_t other;
+    p.pv = locate(tt, g, p.first);
+    p.pk = locate(tt, n >> 2, other);
+    return p;
+  };
+  uint32_t kw[4][KW];
+  u4_t vw[DT];
+  float ks, vs;
+  auto load_keys = [&](uint32_t tt, const Place& p) {
+    const uint32_t slot = (tt * kTokTile + (n >> 2) * 16u) & (bs - 1u);
+    const size_t cell = (size_t)max(p.pk, 0) * a.c.kvh + h;
+    const int8_t* const kp = a.c.k + ((cell << bsh) + slot + (n & 3u)) * D + g * (D / 4);
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
       if constexpr (KW % 4 == 0) {
@@ -182,12 +184,73 @@ __global__ __launch_bounds__(64 * kStepWaves) void k_step(StepArgs a) {
         }
       }
     }
-    const int8_t* vp = a.c.v + ((cell_v * D + n) << bsh) + slot_v;
+  };
+  auto load_values = [&](uint32_t tt, const Place& p) {
+    const uint32_t slot = (tt * kTokTile + g * 16u) & (bs - 1u);
+    const size_t cell = (size_t)max(p.pv, 0) * a.c.kvh + h;
+    const int8_t* const vp = a.c.v + ((cell * D + n) << bsh) + slot;
 #pragma unroll
     for (int t = 0; t < DT; ++t) vw[t] = *reinterpret_cast<const u4_t*>(vp + ((size_t)(16 * t) << bsh));
-    const float ks = pv >= 0 ? a.c.scale[cell_v * 2] * qscale : 0.f;
-    const float vs = pv >= 0 ? a.c.scale[cell_v * 2 + 1] : 0.f;
+  };
+  auto load_scales = [&](const Place& p) {
+    const size_t cell = (size_t)max(p.pv, 0) * a.c.kvh + h;
+    const float2 x = *reinterpret_cast<const float2*>(a.c.scale + cell * 2);
+    ks = p.pv >= 0 ? x.x : 0.f;
+    vs = p.pv >= 0 ? x.y : 0.f;
+  };
 
+  uint32_t tt = split * a.per + wave;
+  const bool any = tt < t_end;
+  Place here, next;
+  if (any) here = place(tt);
+  u4_t raw[KS];
+  {
+    const uint16_t* src = a.q.data + (int64_t)(s.row + tok) * a.q.token_stride + (int64_t)head * a.q.head_stride + g * (D / 4);
+#pragma unroll
+    for (int c = 0; c < KS; ++c) {
+      if constexpr (VEC) {
+        raw[c] = *reinterpret_cast<const u4_t*>(src + 8 * c);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[c][i] = (uint32_t)src[8 * c + 2 * i] | (uint32_t)src[8 * c + 2 * i + 1] << 16;
+      }
+    }
+  }
+  if (any) {
+    load_scales(here);
+    load_keys(tt, here);
+    load_values(tt, here);
+    next = place(tt + W);
+  }
+  // Queries, as f16 with a power of two taken out so that bf16's range fits.
+  h8_t qf[KS];
+  float qscale = a.scale2;
+  if constexpr (BF) {
+    float mag = 0.f;
+#pragma unroll
+    for (int c = 0; c < KS; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mag = fmaxf(mag, finite_abs(load_val<true>((uint16_t)(raw[c][i >> 1] >> (16 * (i & 1))))));
+    mag = rows_max(mag);
+    int e = (int)(__float_as_uint(mag) >> 23) - 127 - 10;  // the largest becomes 2^10 .. 2^11
+    e = e < -100 ? -100 : e;
+    const float inv = exp2_int(-e);
+    qscale *= exp2_int(e);
+#pragma unroll
+    for (int c = 0; c < KS; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        qf[c][i] = (_Float16)(load_val<true>((uint16_t)(raw[c][i >> 1] >> (16 * (i & 1)))) * inv);
+  } else {
+#pragma unroll
+    for (int c = 0; c < KS; ++c) qf[c] = __builtin_bit_cast(h8_t, raw[c]);
+  }
+
+  for (; tt < t_end; tt += W) {
+    // tokens of this lane that its row sees: the first `lim` + 1 of its 16
+    const int32_t lim = here.pv >= 0 && here.first <= pos ? pos - here.first : -1;
+    const float kq = ks * qscale, vcur = vs;
+    const bool more = tt + W < t_end;
     f4_t sc[4];
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
@@ -196,22 +259,24 @@ __global__ __launch_bounds__(64 * kStepWaves) void k_step(StepArgs a) {
       for (int c = 0; c < KS; ++c)
         sc[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(kw[st][2 * c], kw[st][2 * c + 1]), qf[c], sc[st], 0, 0, 0);
     }
-    // tokens of this lane that its row sees: the first `lim` + 1 of its 16
-    const int32_t lim = pv >= 0 && first <= pos ? pos - first : -1;
+    if (more) {
+      load_scales(next);
+      load_keys(tt + W, next);
+    }
     float big = -FLT_MAX;
 #pragma unroll
     for (int st = 0; st < 4; ++st)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float x = sc[st][i] * ks;
+        const float x = sc[st][i] * kq;
         sc[st][i] = 4 * st + i <= lim ? x : -__builtin_inff();
         big = fmaxf(big, sc[st][i]);
       }
-    if (__any(big > M + (kLift + kSlack) || vs > vref)) {
+    if (__any(big > M + (kLift + kSlack) || vcur > vref)) {
       // each row by its own logits alone: a row's result does not depend on its neighbours
       const float row_big = rows_max(big);
       const float m_new = row_big > M + (kLift + kSlack) ? row_big - kLift : M;
-      const float v_new = fmaxf(vref, rows_max(vs));
+      const float v_new = fmaxf(vref, rows_max(vcur));
       const float f = exp2f(M - m_new);
       const float fo = v_new > 0.f ? f * (vref / v_new) : 0.f;
       l *= f;
@@ -223,7 +288,7 @@ __global__ __launch_bounds__(64 * kStepWaves) void k_step(StepArgs a) {
       vref = v_new;
       vinv = v_new > 0.f ? 1.f / v_new : 0.f;
     }
-    const float w = vs * vinv;
+    const float w = vcur * vinv;
     h8_t pf[2];
     float add = 0.f;
 #pragma unroll
@@ -240,6 +305,11 @@ __global__ __launch_bounds__(64 * kStepWaves) void k_step(StepArgs a) {
       acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vw[t].x, vw[t].y), pf[0], acc[t], 0, 0, 0);
       acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vw[t].z, vw[t].w), pf[1], acc[t], 0, 0, 0);
     }
+    if (more) {
+      here = next;
+      next = place(tt + 2 * W);
+      load_values(tt + W, here);
+    }
   }
 
   // The waves' sums meet in LDS, in wave order.
@@ -253,27 +323,24 @@ __global__ __launch_bounds__(64 * kStepWaves) void k_step(StepArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) sm_o[wave][n][16 * t + 4 * g + i] = acc[t][i] * vref;
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < rows * (D / 4); i += 64 * kStepWaves) {
+  for (uint32_t i = threadIdx.x; i < rows * (D / 4); i += 64 * W) {
     const uint32_t rr = i / (D / 4), d = i % (D / 4) * 4;
     float m = sm_m[0][rr];
 #pragma unroll
-    for (uint32_t w = 1; w < kStepWaves; ++w) m = fmaxf(m, sm_m[w][rr]);
+    for (uint32_t w = 1; w < W; ++w) m = fmaxf(m, sm_m[w][rr]);
     float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (uint32_t w = 0; w < kStepWaves; ++w) {
+    for (uint32_t w = 0; w < W; ++w) {
       const float f = exp2f(sm_m[w][rr] - m);
       sum += f * sm_l[w][rr];
 #pragma unroll
       for (int x = 0; x < 4; ++x) o[x] += f * sm_o[w][rr][d + x];
     }
-    const uint32_t rw = r_first + rr;
-    const size_t row = (size_t)(s.row + rw / a.group) * a.q.heads + h * a.group + rw % a.group;
+    const size_t row = row_of(rr);
     if (a.splits > 1) {
-      float* const po = a.part + (row * a.splits + split) * D + d;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) po[x] = o[x];
+      *reinterpret_cast<f4_t*>(a.part + (row * a.splits + split) * D + d) = f4_t{o[0], o[1], o[2], o[3]};
       if (d == 0) {
-        float* const pm = a.part + (size_t)a.b.tokens * a.q.heads * a.splits * D + (row * a.splits + split) * 2;
+        float* const pm = part_ml + (row * a.splits + split) * 2;
         pm[0] = m;
         pm[1] = sum;
       }
@@ -288,43 +355,71 @@ __global__ __launch_bounds__(64 * kStepWaves) void k_step(StepArgs a) {
   }
 }
 
-// Joins the splits of a row; one wave per row.
-template <int D, bool BF>
-__global__ __launch_bounds__(64) void k_join(const float* __restrict__ part, uint32_t splits, uint64_t rows,
-                                             uint16_t* __restrict__ out, float* __restrict__ lse) {
-  const uint64_t row = blockIdx.x;
+// Joins the splits of a row, one workgroup per row: the weights of up to 64
+// splits at a time in the lanes of every wave, the sums of the splits that have
+// any shared out over the waves. (One wave per row that walked its splits took
+// 155 us for 32 rows of 256 splits.)
+template <int D, bool BF, uint32_t W>
+__global__ __launch_bounds__(64 * (W == 1 ? kJoinRows : W)) void k_join(const float* __restrict__ part, uint32_t splits,
+                                                          uint64_t rows, uint16_t* __restrict__ out,
+                                                          float* __restrict__ lse) {
+  constexpr uint32_t L = D / 4;  // lanes that a row of sums takes
+  constexpr uint32_t P = 64 / L > 0 ? 64 / L : 1;
+  __shared__ f4_t sums[W == 1 ? kJoinRows : W][64];
+  const uint32_t lane = threadIdx.x & 63u, wave = W == 1 ? 0u : threadIdx.x >> 6;
+  const uint64_t row = W == 1 ? (uint64_t)blockIdx.x * kJoinRows + (threadIdx.x >> 6) : blockIdx.x;
+  if (W == 1 && row >= rows) return;
   const float* const ml = part + rows * splits * D + row * splits * 2;
+  const float* const po = part + row * splits * D;
   float m = -FLT_MAX;
-  for (uint32_t i = 0; i < splits; ++i) m = fmaxf(m, ml[2 * i]);
-  float sum = 0.f, o[D / 64 + 1];
+  for (uint32_t i = lane; i < splits; i += 64) m = fmaxf(m, ml[2 * i]);
 #pragma unroll
-  for (int x = 0; x <= D / 64; ++x) o[x] = 0.f;
-  for (uint32_t i = 0; i < splits; ++i) {
-    const float f = exp2f(ml[2 * i] - m);
-    sum += f * ml[2 * i + 1];
-    const float* const po = part + (row * splits + i) * D;
+  for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+  float total = 0.f;
+  f4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (uint32_t i0 = 0; i0 < splits; i0 += 64) {
+    const uint32_t i = i0 + lane;
+    const float l = i < splits ? ml[2 * i + 1] : 0.f;
+    const float f = l != 0.f ? exp2f(ml[2 * i] - m) : 0.f;  // a split without sums was not written
+    total += f * l;
+    const uint32_t n = min(64u, splits - i0);
 #pragma unroll
-    for (uint32_t x = 0; x < D; x += 64)
-      if (x + threadIdx.x < D) o[x / 64] += f * po[x + threadIdx.x];
+    for (uint32_t k = wave * P; k < 64; k += W * P) {
+      const uint32_t mine = k + lane / L;
+      const float w = __shfl(f, (int)min(mine, 63u));
+      if (k < n && mine < n && lane < P * L) {
+        const f4_t x = *reinterpret_cast<const f4_t*>(po + (size_t)(i0 + mine) * D + lane % L * 4);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] += w != 0.f ? w * x[c] : 0.f;
+      }
+    }
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
 #pragma unroll
-  for (uint32_t x = 0; x < D; x += 64)
-    if (x + threadIdx.x < D) out[row * D + x + threadIdx.x] = store_val<BF>(sum == 0.f ? 0.f : o[x / 64] * inv);
-  if (lse && threadIdx.x == 0) lse[row] = sum == 0.f ? -__builtin_inff() : (m + log2f(sum)) * kLn2;
-}
-
-// How many workgroups share a row tile's tokens.
-uint32_t split_rule(uint64_t units, uint64_t tokens) {
-  const uint64_t most = (tokens + kStepWaves * kTokTile - 1) / (kStepWaves * kTokTile);  // a tile for every wave
-  const uint64_t want = (kSplitUnits + units - 1) / (units ? units : 1);
-  const uint64_t n = want < most ? want : most;
-  return n < 1 ? 1u : n > 256 ? 256u : (uint32_t)n;
+  for (int x = 1; x < 64; x <<= 1) total += __shfl_xor(total, x);
+  f4_t* const mine = sums[W == 1 ? threadIdx.x >> 6 : 0];  // W == 1: the wave's own, in program order
+  sums[threadIdx.x >> 6][lane] = o;
+  if constexpr (W > 1) __syncthreads();
+  if (wave == 0 && lane < L) {
+    f4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w)
+#pragma unroll
+      for (uint32_t p = 0; p < P; ++p)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) y[c] += mine[w * 64 + p * L + lane][c];
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+    uint16_t z[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) z[c] = store_val<BF>(total == 0.f ? 0.f : y[c] * inv);
+    *reinterpret_cast<u2_t*>(out + row * D + lane * 4) = u2_t{z[0] | (uint32_t)z[1] << 16, z[2] | (uint32_t)z[3] << 16};
+    if (lse && lane == 0) lse[row] = total == 0.f ? -__builtin_inff() : (m + log2f(total)) * kLn2;
+  }
 }
 
 struct Plan {
   uint64_t units;  // sequences or token rows, x row tiles x kv heads
-  uint32_t tiles, splits;
+  uint32_t tiles, splits, per;
+  bool wide;
   size_t work;
 };
 Plan plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, bool list, uint32_t count) {
@@ -334,7 +429,19 @@ Plan plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, bool lis
   const uint64_t rows = list ? group : group * b->max_tokens;
   p.tiles = (uint32_t)((rows + kRowTile - 1) / kRowTile);
   p.units = (uint64_t)(list ? b->tokens : b->seqs) * p.tiles * c->kv_heads;
-  p.splits = split_rule(p.units, (uint64_t)(list ? count : most_blocks(c, b)) * c->block_tokens);
+  // A split takes a fixed number of tiles, so that sequences of other lengths take
+  // other numbers of workgroups.
+  const uint64_t all = ((uint64_t)(list ? count : most_blocks(c, b)) * c->block_tokens + kTokTile - 1) / kTokTile;
+  p.wide = p.units <= kWideUnits && all * kTokTile * 2 * c->dim <= kWideBytes;
+  if (p.wide) {
+    p.per = (uint32_t)all;
+    p.splits = 1;
+    return p;
+  }
+  uint64_t per = (p.units * all + kSplitUnits - 1) / kSplitUnits;
+  per = per < kSplitTiles ? kSplitTiles : (per + kStepWaves - 1) / kStepWaves * kStepWaves;
+  p.per = (uint32_t)(per < all ? per : all);
+  p.splits = (uint32_t)((all + p.per - 1) / p.per);
   if (p.splits > 1) p.work = (size_t)b->tokens * heads * p.splits * (c->dim + 2) * 4;
   return p;
 }
@@ -359,29 +466,37 @@ int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, c
     return -1;
   }
   const uint64_t grid = p.units * p.splits;
-  if (grid * 64 * kStepWaves > 0xFFFFFFFFull || (uint64_t)batch->tokens * q->heads * 64 > 0xFFFFFFFFull) {
+  if (grid * 64 * kStepWaves > 0xFFFFFFFFull || (uint64_t)batch->tokens * q->heads * 64 * kJoinWaves > 0xFFFFFFFFull) {
     std::fprintf(stderr, "[%s] batch is too large for one launch\n", who);
     return -1;
   }
   const hipStream_t st = static_cast<hipStream_t>(stream);
   StepArgs a{cache_args(cache), batch_args(batch), rows_args(q), lists, count, scale * kLog2e,
-             q->heads / cache->kv_heads, p.tiles, p.splits, static_cast<uint16_t*>(out), lse,
+             q->heads / cache->kv_heads, p.tiles, list ? batch->tokens : batch->seqs, p.splits, p.per, static_cast<uint16_t*>(out), lse,
              static_cast<float*>(work)};
   const bool vec = rows_vector(q);
   with_kind(cache->dim, q->dtype, [&](auto d, auto bf) {
     constexpr int D = decltype(d)::value;
     constexpr bool BF = decltype(bf)::value;
     auto go = [&](auto l, auto v) {
-      hipLaunchKernelGGL((k_step<D, BF, decltype(l)::value, decltype(v)::value>), dim3((uint32_t)grid),
-                         dim3(64 * kStepWaves), 0, st, a);
+      constexpr bool L = decltype(l)::value, V = decltype(v)::value;
+      constexpr uint32_t W = wide_waves(D);
+      if (p.wide)
+        hipLaunchKernelGGL((k_step<D, BF, L, V, W>), dim3((uint32_t)grid), dim3(64 * W), 0, st, a);
+      else
+        hipLaunchKernelGGL((k_step<D, BF, L, V, kStepWaves>), dim3((uint32_t)grid), dim3(64 * kStepWaves), 0, st, a);
     };
     if (list)
       vec ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
     else
       vec ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
-    if (p.splits > 1)
-      hipLaunchKernelGGL((k_join<D, BF>), dim3(batch->tokens * q->heads), dim3(64), 0, st, a.part, p.splits,
-                         (uint64_t)batch->tokens * q->heads, a.out, lse);
+    const uint64_t rows = (uint64_t)batch->tokens * q->heads;
+    if (p.splits > kJoinFew)
+      hipLaunchKernelGGL((k_join<D, BF, kJoinWaves>), dim3((uint32_t)rows), dim3(64 * kJoinWaves), 0, st, a.part,
+                         p.splits, rows, a.out, lse);
+    else if (p.splits > 1)
+      hipLaunchKernelGGL((k_join<D, BF, 1>), dim3((uint32_t)((rows + kJoinRows - 1) / kJoinRows)),
+                         dim3(64 * kJoinRows), 0, st, a.part, p.splits, rows, a.out, lse);
   });
   return launched(who);
 }

@@ -83,6 +83,14 @@ __device__ __forceinline__ uint32_t seq_at(const Batch& b, uint32_t row) {
   return lo;
 }
 
+// a - b, or 0 where b is more; both below 2^31. In signed numbers: the compiler
+// (ROCm 7.2) turns an unsigned difference that stops at 0 of two scalars into s_sub
+// without the stop.
+__device__ __forceinline__ uint32_t less(uint32_t a, uint32_t b) {
+  const int32_t d = (int32_t)a - (int32_t)b;
+  return d > 0 ? (uint32_t)d : 0u;
+}
+
 template <bool BF>
 __device__ __forceinline__ float load_val(uint16_t u) {
   if constexpr (BF)
@@ -137,6 +145,11 @@ __device__ __forceinline__ h8_t codes8(uint32_t a, uint32_t b) {
 __device__ __forceinline__ float rows_max(float x) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+// Over the two lanes that differ in bit 4.
+__device__ __forceinline__ float pair_max(float x) {
   const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }

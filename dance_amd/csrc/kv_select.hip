@@ -5,12 +5,17 @@
 // dimension, c k <= max(c hi, c lo) for the code c of the query and each of the
 // block's codes k: c hi where c > 0, c lo where c < 0. The bound of all
 // dimensions is thus one product of length 2 D, (c+ | c-) with (hi | lo), the
-// latter as they lie in memory. It is done with 16x16x64 i8 MFMAs, 16 blocks by
-// 16 query rows, exactly; only the block's scale is rounded in (once).
+// latter as they lie in memory. It is done with 16x16x64 i8 MFMAs, 16 query rows
+// by 16 blocks, exactly; only the block's scale is rounded in (once). The
+// result registers of a lane are four rows of one block: with groups of up to
+// four heads the group's largest score needs no other lane.
 //
-// Choice: the count-th largest key by its 8-bit digits from the top (counts
-// in LDS), then one pass in index order that keeps what is larger, and of what
-// equals it the first ones.
+// The scores of a few token rows stay in LDS as whole numbers that order like
+// them, and the same workgroup chooses: it counts the keys by 8 bits of their
+// distance from the least, which spreads them over the counters whatever
+// their exponents are, narrows the range to the counter that holds the
+// count-th largest until it is all taken or a single key, and writes what
+// is larger, and of what equals it the first ones, in index order.
 
 #include <cmath>
 #include <type_traits>
@@ -21,192 +26,443 @@ namespace dance {
 namespace kv {
 namespace {
 
-constexpr uint32_t kScoreWaves = 4;
-constexpr uint32_t kTopThreads = 256;
+constexpr uint32_t kSelWaves = 8;
+constexpr uint32_t kSelThreads = 64 * kSelWaves;
+constexpr uint32_t kTwo = 2;  // block tiles of 16 that a wave has on the way at once
+
+constexpr uint32_t kNoKey = 0x007FFFFFu;   // of -inf: holes
+constexpr uint32_t kForced = 0xFFFFFFFFu;  // above all scores
+__device__ __forceinline__ uint32_t sort_key(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
 
 struct SelectArgs {
   Cache c;
   Batch b;
   Rows q;
-  uint32_t group, count, sink, recent;
-  uint32_t stride;  // scores of a (token row, kv head)
-  float* __restrict__ score;
+  uint32_t group, gp;    // heads of a kv head; padded to a power of two where they share a row tile
+  uint32_t ntok, tiles;  // token rows of a workgroup, workgroups of a sequence
+  uint32_t count, sink, recent;
+  uint32_t blocks;       // keys of a token row
+  uint32_t chunks, per;  // k_score: workgroups that share the blocks, blocks of each
+  uint32_t* __restrict__ keys;  // where they do not stay in LDS: [token row][kv head][blocks]
   int32_t* __restrict__ chosen;
 };
 
-// Position of a token row and the blocks it sees; none for a row of no sequence.
-struct Place {
-  uint32_t sq, seen;
-};
-__device__ __forceinline__ Place place_of(const SelectArgs& a, uint32_t row) {
-  Place p;
-  p.sq = seq_at(a.b, row);
-  const Seq s = seq_of(a.b, p.sq, a.c.bsh);
-  p.seen = 0;
-  if (row >= s.row && row - s.row < s.n) {
-    const int64_t at = s.first + (row - s.row);
-    const int64_t end = at + 1 < s.len ? at + 1 : s.len;
-    if (end > 0) p.seen = min((uint32_t)((end + (1ll << a.c.bsh) - 1) >> a.c.bsh), a.stride);
+// The token rows of a workgroup and what they see.
+struct Tokens {
+  uint32_t sq, row, n;  // sequence, first row, rows
+  int64_t first;        // position of the first row
+  int64_t len;
+  __device__ __forceinline__ uint32_t seen(const SelectArgs& a, uint32_t t) const {
+    const int64_t end = first + t + 1 < len ? first + t + 1 : len;
+    return end > 0 ? min((uint32_t)((end + (1ll << a.c.bsh) - 1) >> a.c.bsh), a.blocks) : 0u;
   }
-  return p;
+};
+__device__ __forceinline__ Tokens tokens_of(const SelectArgs& a, uint32_t sq, uint32_t tile) {
+  const Seq s = seq_of(a.b, sq, a.c.bsh);
+  const uint32_t t0 = tile * a.ntok;
+  return Tokens{sq, s.row + t0, min(a.ntok, less(s.n, t0)), s.first + t0, s.len};
 }
 
-template <int D, bool BF>
-__global__ __launch_bounds__(64 * kScoreWaves) void k_score(SelectArgs a, uint32_t chunks, uint32_t per) {
+constexpr int kRowTiles = 4;  // row tiles that a pass over the blocks serves
+template <int D>
+struct Codes {
+  // Row stride: 16 bytes over the codes, so that the 16 rows of an operand lie in
+  // different banks.
+  static constexpr uint32_t kStride = 2 * D + 16;
+  int8_t c[kRowTiles * 16 * kStride];
+  float up[kRowTiles * 16];  // 2^e of a row's codes; 0: no row
+};
+
+// Codes of row tiles [p0, p0 + kRowTiles): a wave's four lane groups of 16 take a row each.
+template <int D, bool BF, bool VEC>
+__device__ __forceinline__ void code_rows(const SelectArgs& a, const Tokens& tk, uint32_t h, uint32_t p0, uint32_t rows,
+                                          Codes<D>& qc) {
+  constexpr int V = D / 16;  // values of a lane; 8 at a time where they are 8 or 16
+  const uint32_t l = threadIdx.x & 15u;
+  const uint32_t end = min((uint32_t)kRowTiles, rows - p0) * 16u;
+  for (uint32_t r = threadIdx.x >> 4; r < end; r += kSelThreads / 16) {
+    const uint32_t t = a.group > 16u ? 0u : (p0 * 16u + r) / a.gp;
+    const uint32_t f = a.group > 16u ? p0 * 16u + r : r % a.gp;
+    const bool live = t < tk.n && f < a.group;
+    const uint16_t* const src = a.q.data + (int64_t)(tk.row + (live ? t : 0u)) * a.q.token_stride +
+                                (int64_t)(h * a.group + (live ? f : 0u)) * a.q.head_stride + l * V;
+    float x[V];
+    if constexpr (VEC && V % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i) {
+        const u2_t w = *reinterpret_cast<const u2_t*>(src + 4 * i);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) x[4 * i + b] = load_val<BF>((uint16_t)(w[b >> 1] >> (16 * (b & 1))));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[i] = load_val<BF>(src[i]);
+    }
+    float mag = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) mag = fmaxf(mag, finite_abs(x[i]));
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) mag = fmaxf(mag, __shfl_xor(mag, d));
+    const int e = scale_exp(mag);
+    const float inv = exp2_int(-e);
+    int8_t* const out = qc.c + r * Codes<D>::kStride + l * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int code = code_of(x[i], inv);
+      out[i] = (int8_t)max(code, 0);
+      out[D + i] = (int8_t)min(code, 0);
+    }
+    if (l == 0) qc.up[r] = live ? exp2_int(e) : 0.f;
+  }
+}
+
+// Keys of blocks [from, to) for the workgroup's token rows: keys[t * stride + block].
+template <int D, bool BF, bool VEC>
+__device__ __forceinline__ void score_blocks(const SelectArgs& a, const Tokens& tk, uint32_t h, uint32_t from,
+                                             uint32_t to, uint32_t* __restrict__ keys, size_t stride, Codes<D>& qc) {
   constexpr int KS = D / 32;  // inner steps of 64 over 2 D
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const uint32_t n = lane & 15u, g = lane >> 4;
-  uint32_t id = blockIdx.x;
-  const uint32_t chunk = id % chunks;
-  id /= chunks;
-  const uint32_t h = id % a.c.kvh, row = id / a.c.kvh;
-  const Place p = place_of(a, row);
-  const uint32_t first = chunk * per, end = min(first + per, p.seen);
-  if (first >= end) return;
-  const int32_t* const table = a.b.table + (size_t)p.sq * a.b.width;
-  float* const out = a.score + ((size_t)row * a.c.kvh + h) * a.stride;
-  const uint32_t forced = p.seen > a.recent ? p.seen - a.recent : 0u;
-
-  for (uint32_t r0 = 0; r0 < a.group; r0 += 16) {
-    // This lane's part of its row's codes: positive part in lane groups 0 and 1
-    // (against hi), negative part in 2 and 3 (against lo).
-    const uint32_t r = r0 + n;
-    const bool live = r < a.group;
-    const uint16_t* const src = a.q.data + (int64_t)row * a.q.token_stride +
-                                (int64_t)(h * a.group + (live ? r : 0u)) * a.q.head_stride + (g & 1u) * (D / 2);
-    float mag = 0.f;
-    for (int i = 0; i < D / 2; ++i) mag = fmaxf(mag, finite_abs(load_val<BF>(src[i])));
-    mag = rows_max(mag);
-    const int e = scale_exp(mag);
-    const float inv = exp2_int(-e), up = exp2_int(e);
-    i4_t qf[KS];
-#pragma unroll
-    for (int c = 0; c < KS; ++c)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t x = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const int code = code_of(load_val<BF>(src[16 * c + 4 * w + b]), inv);
-          const int part = g < 2 ? max(code, 0) : min(code, 0);
-          x |= (uint32_t)(part & 255) << (8 * b);
-        }
-        qf[c][w] = (int)x;
-      }
-    for (uint32_t b0 = first + wave * 16; b0 < end; b0 += kScoreWaves * 16) {
-      const uint32_t mine = b0 + n;  // the block that this lane loads for
-      int32_t ph = mine < end ? table[mine] : -1;
-      if ((uint32_t)ph >= a.c.blocks) ph = -1;
-      const size_t cell = (size_t)max(ph, 0) * a.c.kvh + h;
+  const int32_t* const table = a.b.table + (size_t)tk.sq * a.b.width;
+  const uint32_t per_tile = 16u / a.gp;  // token rows of a row tile
+  const uint32_t rows = a.group > 16u ? (a.group + 15u) / 16u : (tk.n + per_tile - 1u) / per_tile;
+  for (uint32_t p0 = 0; p0 < rows; p0 += kRowTiles) {
+    if (p0) __syncthreads();
+    code_rows<D, BF, VEC>(a, tk, h, p0, rows, qc);
+    __syncthreads();
+    const uint32_t here = min((uint32_t)kRowTiles, rows - p0);
+    struct Tile {
+      i4_t b[KS];
+      int32_t ph;
+      float ks;
+    };
+    auto load = [&](uint32_t blk) {
+      Tile t;
+      t.ph = blk < to ? table[blk] : -1;
+      if ((uint32_t)t.ph >= a.c.blocks) t.ph = -1;
+      const size_t cell = (size_t)max(t.ph, 0) * a.c.kvh + h;
       const int8_t* const bp = a.c.bound + cell * 2 * D + g * (D / 2);
-      const float ks = ph >= 0 ? a.c.scale[cell * 2] : 0.f;
+#pragma unroll
+      for (int c = 0; c < KS; ++c) t.b[c] = *reinterpret_cast<const i4_t*>(bp + 16 * c);
+      t.ks = a.c.scale[cell * 2];
+      return t;
+    };
+    auto put = [&](uint32_t t, uint32_t blk, bool hole, float x, bool add) {
+      if (t >= tk.n || blk >= to) return;
+      const uint32_t seen = tk.seen(a, t);
+      uint32_t key = sort_key(x + 0.f);
+      if (blk < a.sink || blk + a.recent >= seen) key = kForced;
+      if (hole) key = kNoKey;
+      uint32_t* const at = keys + t * stride + blk;
+      *at = add ? max(key, *at) : key;  // more than 16 heads: the same lane's key of those before
+    };
+    auto score = [&](const Tile& b, uint32_t blk, uint32_t r, const i4_t* qf, const float* up) {
       i4_t acc = {0, 0, 0, 0};
 #pragma unroll
-      for (int c = 0; c < KS; ++c)
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const i4_t*>(bp + 16 * c), qf[c], acc, 0, 0, 0);
+      for (int c = 0; c < KS; ++c) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf[c], b.b[c], acc, 0, 0, 0);
+      float x[4];  // rows 4 g + i of block n
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t m = 4 * g + i;  // block b0 + m, held by lane m
-        const float sc = __shfl(ks, (int)m);
-        const bool hole = __shfl(ph, (int)m) < 0;
-        float x = live ? ((float)acc[i] * sc) * up + 0.f : -__builtin_inff();
+      for (int i = 0; i < 4; ++i) x[i] = up[i] > 0.f ? ((float)acc[i] * b.ks) * up[i] : -__builtin_inff();
+      const bool hole = b.ph < 0;
+      const uint32_t t0 = (p0 + r) * per_tile;
+      if (a.group > 16u) {
+        const float m = rows_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+        if (g == 0) put(0, blk, hole, m, p0 + r != 0);
+      } else if (a.gp == 1) {
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) x = fmaxf(x, __shfl_xor(x, d));
-        const uint32_t blk = b0 + m;
-        if (n == 0 && blk < end) {
-          if (r0) x = fmaxf(x, out[blk]);
-          if (blk < a.sink || blk >= forced) x = __builtin_inff();
-          out[blk] = hole ? -__builtin_inff() : x;
+        for (int i = 0; i < 4; ++i) put(t0 + 4 * g + i, blk, hole, x[i], false);
+      } else if (a.gp == 2) {
+        put(t0 + 2 * g, blk, hole, fmaxf(x[0], x[1]), false);
+        put(t0 + 2 * g + 1, blk, hole, fmaxf(x[2], x[3]), false);
+      } else {
+        float m = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        if (a.gp == 4) {
+          put(t0 + g, blk, hole, m, false);
+        } else if (a.gp == 8) {
+          m = pair_max(m);
+          if ((g & 1u) == 0) put(t0 + (g >> 1), blk, hole, m, false);
+        } else {
+          m = rows_max(m);
+          if (g == 0) put(t0, blk, hole, m, false);
         }
       }
+    };
+    constexpr uint32_t kStep = kSelWaves * kTwo * 16u;
+    Tile cur[kTwo];
+    uint32_t blk = from + wave * kTwo * 16u + n;
+    if (blk - n < to)
+#pragma unroll
+      for (uint32_t u = 0; u < kTwo; ++u) cur[u] = load(blk + 16u * u);
+    for (; blk - n < to; blk += kStep) {
+      Tile nxt[kTwo];
+      const bool more = blk - n + kStep < to;
+      if (more)
+#pragma unroll
+        for (uint32_t u = 0; u < kTwo; ++u) nxt[u] = load(blk + kStep + 16u * u);
+      for (uint32_t r = 0; r < here; ++r) {
+        i4_t qf[KS];
+        float up[4];
+#pragma unroll
+        for (int c = 0; c < KS; ++c)
+          qf[c] = *reinterpret_cast<const i4_t*>(qc.c + (r * 16u + n) * Codes<D>::kStride + g * (D / 2) + 16 * c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) up[i] = qc.up[r * 16u + 4 * g + i];
+#pragma unroll
+        for (uint32_t u = 0; u < kTwo; ++u) score(cur[u], blk + 16u * u, r, qf, up);
+      }
+      if (more)
+#pragma unroll
+        for (uint32_t u = 0; u < kTwo; ++u) cur[u] = nxt[u];
     }
   }
 }
 
-__device__ __forceinline__ uint32_t sort_key(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-constexpr uint32_t kNoKey = 0x007FFFFFu;  // sort_key(-inf): holes
+// What a team of W waves shares while it chooses.
+struct Team {
+  uint32_t hist[256];
+  uint32_t lo, hi, digit, left;          // W > 1
+  uint32_t more[kSelWaves], same[kSelWaves], forced[kSelWaves];
+};
 
-__global__ __launch_bounds__(kTopThreads) void k_top(SelectArgs a) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t pick[2];
-  __shared__ uint32_t wave_more[kTopThreads / 64], wave_same[kTopThreads / 64];
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-  const uint32_t h = blockIdx.x % a.c.kvh, row = blockIdx.x / a.c.kvh;
-  const Place p = place_of(a, row);
-  const float* const score = a.score + ((size_t)row * a.c.kvh + h) * a.stride;
-  int32_t* const out = a.chosen + ((size_t)row * a.c.kvh + h) * a.count;
-  // Digits from the top: `want` of the keys that share the prefix are still to be found.
-  uint32_t prefix = 0, want = a.count;
-  bool all = p.seen <= a.count;
-  for (int shift = 24; shift >= 0 && !all; shift -= 8) {
-    hist[tid] = 0;
-    __syncthreads();
-    const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-    for (uint32_t i = tid; i < p.seen; i += kTopThreads) {
-      const uint32_t k = sort_key(score[i]);
-      if ((k & mask) == prefix) atomicAdd(&hist[k >> shift & 255u], 1u);
+// The `count` blocks of the n with the largest keys, ties to the lower block, ascending.
+template <uint32_t W>
+__device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32_t n, uint32_t count,
+                                       int32_t* __restrict__ out, Team& tm) {
+  const uint32_t lane = threadIdx.x & 63u, wave = W == 1 ? 0u : threadIdx.x >> 6;
+  const uint32_t tid = W == 1 ? lane : threadIdx.x;
+  auto sync = [&] {
+    if constexpr (W > 1) {
+      __syncthreads();
+    } else {  // a wave's LDS accesses complete in order; the compiler has to keep it
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
-    __syncthreads();
-    if (wave == 0) {
-      // lane i sums digits 4 i .. 4 i + 3, then counts from the largest digit down
-      const uint32_t c0 = hist[4 * lane], c1 = hist[4 * lane + 1], c2 = hist[4 * lane + 2], c3 = hist[4 * lane + 3];
-      const uint32_t mine = c0 + c1 + c2 + c3;
-      uint32_t above = mine;  // becomes the sum over this lane and those after it
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_down(above, d);
-        if (lane + d < 64) above += o;
-      }
-      above -= mine;
-      if (above < want && above + mine >= want) {
-        uint32_t left = want - above, digit = 4 * lane + 3;
-        if (left > c3) left -= c3, digit = 4 * lane + 2;
-        if (digit == 4 * lane + 2 && left > c2) left -= c2, digit = 4 * lane + 1;
-        if (digit == 4 * lane + 1 && left > c1) left -= c1, digit = 4 * lane;
-        pick[0] = digit;
-        pick[1] = left;
-      }
+  };
+  // Range of the keys that compete, how many they are, and how many are forced.
+  uint32_t lo = ~0u, hi = 0, some = 0, forced = 0;
+  for (uint32_t i = tid; i < n; i += 64 * W) {
+    const uint32_t k = keys[i];
+    if (k == kForced) {
+      ++forced;
+    } else if (k > kNoKey) {
+      lo = min(lo, k);
+      hi = max(hi, k);
+      ++some;
     }
-    __syncthreads();
-    prefix |= pick[0] << shift;
-    want = pick[1];
-    __syncthreads();
   }
-  // Keys above the limit, and the first `want` that equal it; no hole.
-  const uint32_t limit = all ? kNoKey : max(prefix, kNoKey);
-  if (limit == kNoKey) want = 0;
-  uint32_t done = 0, same_done = 0;
-  for (uint32_t i0 = 0; i0 < p.seen; i0 += kTopThreads) {
-    const uint32_t i = i0 + tid;
-    const uint32_t k = i < p.seen ? sort_key(score[i]) : 0u;
-    const bool same = k == limit && i < p.seen;
-    const uint64_t same_mask = __ballot(same);
-    const uint64_t below = (1ull << lane) - 1;
-    if (lane == 0) wave_same[wave] = (uint32_t)__popcll(same_mask);
-    __syncthreads();
-    uint32_t rank = same_done + (uint32_t)__popcll(same_mask & below);
 #pragma unroll
-    for (uint32_t w = 0; w < kTopThreads / 64; ++w) {
-      if (w < wave) rank += wave_same[w];
-      same_done += wave_same[w];
-    }
-    const bool take = k > limit || (same && rank < want);
-    const uint64_t take_mask = __ballot(take);
-    if (lane == 0) wave_more[wave] = (uint32_t)__popcll(take_mask);
-    __syncthreads();
-    uint32_t at = done + (uint32_t)__popcll(take_mask & below);
-#pragma unroll
-    for (uint32_t w = 0; w < kTopThreads / 64; ++w) {
-      if (w < wave) at += wave_more[w];
-      done += wave_more[w];
-    }
-    if (take && at < a.count) out[at] = (int32_t)i;
-    __syncthreads();
+  for (int d = 1; d < 64; d <<= 1) {
+    lo = min(lo, (uint32_t)__shfl_xor((int)lo, d));
+    hi = max(hi, (uint32_t)__shfl_xor((int)hi, d));
+    some += (uint32_t)__shfl_xor((int)some, d);
+    forced += (uint32_t)__shfl_xor((int)forced, d);
   }
-  for (uint32_t i = done + tid; i < a.count; i += kTopThreads) out[i] = -1;
+  if constexpr (W > 1) {
+    if (tid == 0) tm.lo = ~0u, tm.hi = 0;
+    if (lane == 0) tm.more[wave] = some, tm.forced[wave] = forced;
+    __syncthreads();
+    if (lane == 0) atomicMin(&tm.lo, lo), atomicMax(&tm.hi, hi);
+    some = forced = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w) some += tm.more[w], forced += tm.forced[w];
+    __syncthreads();
+    lo = tm.lo, hi = tm.hi;
+  }
+  // All keys above `limit` are taken, and the first `ties` equal to it.
+  uint32_t want = less(count, forced), limit, ties = 0;
+  if (some <= want) {
+    limit = kNoKey;
+  } else if (want == 0) {
+    limit = kForced - 1u;
+  } else {
+    while (true) {
+      const uint32_t bits = 32u - (uint32_t)__clz((int)(hi - lo | 1u));
+      const uint32_t shift = less(bits, 8u);
+      for (uint32_t i = tid; i < 256; i += 64 * W) tm.hist[i] = 0;
+      sync();
+      for (uint32_t i = tid; i < n; i += 64 * W) {
+        const uint32_t k = keys[i];
+        if (k >= lo && k <= hi) atomicAdd(&tm.hist[(k - lo) >> shift], 1u);
+      }
+      sync();
+      uint32_t digit = 0, left = 0;
+      if (W == 1 || wave == 0) {
+        // lane i has counters 4 i .. 4 i + 3; counted from the largest down
+        uint32_t c[4], mine = 0;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) c[x] = tm.hist[4 * lane + x], mine += c[x];
+        uint32_t from = mine;  // over this lane and those after it
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+          const uint32_t o = (uint32_t)__shfl_down((int)from, d);
+          if (lane + d < 64) from += o;
+        }
+        uint32_t above = from - mine;
+        const bool here = above < want && from >= want;
+        uint32_t dg = 0, rest = 0, full = 0;
+#pragma unroll
+        for (int x = 3; x >= 0; --x) {
+          if (above < want && above + c[x] >= want) dg = 4 * lane + x, rest = want - above, full = c[x] == rest;
+          above += c[x];
+        }
+        const int src = __ffsll((unsigned long long)__ballot(here)) - 1;
+        digit = (uint32_t)__shfl((int)dg, src);
+        left = (uint32_t)__shfl((int)rest, src) | (uint32_t)__shfl((int)full, src) << 31;
+      }
+      if constexpr (W > 1) {
+        if (tid == 0) tm.digit = digit, tm.left = left;
+        __syncthreads();
+        digit = tm.digit, left = tm.left;
+        __syncthreads();
+      }
+      lo += digit << shift;
+      want = left & 0x7FFFFFFFu;
+      if (left >> 31) {  // all of this counter's keys
+        limit = lo - 1u;
+        break;
+      }
+      if (shift == 0) {
+        limit = lo;
+        ties = want;
+        break;
+      }
+      hi = lo + min(hi - lo, (1u << shift) - 1u);
+    }
+  }
+  // Each wave takes its part of the blocks, in order.
+  const uint32_t part = ((n + W - 1) / W + 63u) & ~63u;
+  const uint32_t b0 = min(n, wave * part), b1 = min(n, b0 + part);
+  uint32_t at = 0, rank = 0;
+  if constexpr (W > 1) {
+    uint32_t more = 0, same = 0;
+    for (uint32_t i = b0 + lane; i < b1; i += 64) {
+      const uint32_t k = keys[i];
+      more += k > limit;
+      same += k == limit;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) more += (uint32_t)__shfl_xor((int)more, d), same += (uint32_t)__shfl_xor((int)same, d);
+    if (lane == 0) tm.more[wave] = more, tm.same[wave] = same;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w)
+      if (w < wave) at += tm.more[w] + min(tm.same[w], less(ties, rank)), rank += tm.same[w];
+  }
+  const uint64_t below = (1ull << lane) - 1;
+  for (uint32_t i0 = b0; i0 < b1; i0 += 64) {
+    const uint32_t i = i0 + lane;
+    const uint32_t k = i < b1 ? keys[i] : 0u;
+    const uint64_t same = __ballot(i < b1 && k == limit);
+    const uint32_t r = rank + (uint32_t)__popcll(same & below);
+    const bool take = i < b1 && (k > limit || (k == limit && r < ties));
+    const uint64_t got = __ballot(take);
+    const uint32_t pos = at + (uint32_t)__popcll(got & below);
+    if (take && pos < count) out[pos] = (int32_t)i;
+    rank += (uint32_t)__popcll(same);
+    at += (uint32_t)__popcll(got);
+  }
+  // -1 behind them
+  uint32_t total = at;
+  if constexpr (W > 1) {
+    __syncthreads();
+    if (wave == W - 1 && lane == 0) tm.lo = at;
+    __syncthreads();
+    total = tm.lo;
+  }
+  for (uint32_t i = total + tid; i < count; i += 64 * W) out[i] = -1;
+  sync();
+}
+
+// Scores in LDS, chosen by the workgroup that made them.
+template <int D, bool BF, bool VEC>
+__global__ __launch_bounds__(kSelThreads) void k_select(SelectArgs a) {
+  extern __shared__ uint32_t lds_keys[];
+  __shared__ Team teams[kSelWaves];
+  __shared__ __attribute__((aligned(16))) Codes<D> codes;
+  uint32_t id = blockIdx.x;
+  const uint32_t h = id % a.c.kvh;
+  id /= a.c.kvh;
+  const Tokens tk = tokens_of(a, id / a.tiles, id % a.tiles);
+  if (tk.n == 0) return;
+  score_blocks<D, BF, VEC>(a, tk, h, 0, tk.seen(a, tk.n - 1), lds_keys, a.blocks, codes);
+  __syncthreads();
+  const size_t out = ((size_t)tk.row * a.c.kvh + h) * a.count;
+  if (a.ntok == 1) {
+    choose<kSelWaves>(lds_keys, tk.seen(a, 0), a.count, a.chosen + out, teams[0]);
+  } else {
+    const uint32_t wave = threadIdx.x >> 6;
+    for (uint32_t t = wave; t < tk.n; t += kSelWaves)
+      choose<1>(lds_keys + (size_t)t * a.blocks, tk.seen(a, t), a.count,
+                a.chosen + out + (size_t)t * a.c.kvh * a.count, teams[wave]);
+  }
+}
+
+// Scores to memory, the blocks shared out over workgroups.
+template <int D, bool BF, bool VEC>
+__global__ __launch_bounds__(kSelThreads) void k_score(SelectArgs a) {
+  __shared__ __attribute__((aligned(16))) Codes<D> codes;
+  uint32_t id = blockIdx.x;
+  const uint32_t h = id % a.c.kvh;
+  id /= a.c.kvh;
+  const uint32_t chunk = id % a.chunks;
+  id /= a.chunks;
+  const Tokens tk = tokens_of(a, id / a.tiles, id % a.tiles);
+  if (tk.n == 0) return;
+  const uint32_t from = chunk * a.per, to = min(tk.seen(a, tk.n - 1), from + a.per);
+  if (from < to)
+    score_blocks<D, BF, VEC>(a, tk, h, from, to, a.keys + ((size_t)tk.row * a.c.kvh + h) * a.blocks,
+                             (size_t)a.c.kvh * a.blocks, codes);
+}
+
+__global__ __launch_bounds__(kSelThreads) void k_top(SelectArgs a) {
+  __shared__ Team team;
+  const uint32_t h = blockIdx.x % a.c.kvh;
+  const uint32_t row = blockIdx.x / a.c.kvh;
+  const uint32_t sq = seq_at(a.b, row);
+  const Seq s = seq_of(a.b, sq, a.c.bsh);
+  if (row < s.row || row - s.row >= s.n) return;
+  const Tokens tk{sq, row, 1, s.first + (row - s.row), s.len};
+  const size_t unit = (size_t)row * a.c.kvh + h;
+  choose<kSelWaves>(a.keys + unit * a.blocks, tk.seen(a, 0), a.count, a.chosen + unit * a.count, team);
+}
+
+}  // namespace
+}  // namespace kv
+}  // namespace dance
+
+namespace dance {
+namespace kv {
+namespace {
+
+// Keys that a workgroup may keep: 96 KB, so that its counters and others' LDS fit beside it.
+constexpr uint64_t kLdsKeys = 24576;
+// A few long rows: scores by many workgroups, to memory and back.
+constexpr uint64_t kFewUnits = 64, kManyBlocks = 2048;
+
+struct SelectPlan {
+  bool fused;
+  uint32_t gp, ntok, tiles, blocks;
+  uint64_t groups;  // workgroups over sequences and kv heads
+};
+SelectPlan select_plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads) {
+  SelectPlan p{};
+  const uint32_t group = heads / c->kv_heads;
+  p.gp = 1;
+  while (p.gp < group && p.gp < 16) p.gp *= 2;
+  p.blocks = most_blocks(c, b);
+  uint64_t ntok = group > 16 ? 1 : (uint64_t)kRowTiles * (16 / p.gp);
+  if (ntok > b->max_tokens) ntok = b->max_tokens;
+  const uint64_t units = (uint64_t)b->seqs * c->kv_heads;
+  p.fused = p.blocks <= kLdsKeys && !(b->max_tokens == 1 && units < kFewUnits && p.blocks > kManyBlocks);
+  if (p.fused && ntok * p.blocks > kLdsKeys) ntok = kLdsKeys / p.blocks;
+  p.ntok = (uint32_t)ntok;
+  p.tiles = (uint32_t)((b->max_tokens + ntok - 1) / ntok);
+  p.groups = units * p.tiles;
+  return p;
 }
 
 }  // namespace
@@ -218,8 +474,9 @@ using namespace dance::kv;
 extern "C" {
 
 size_t dance_kv_select_work(const DanceKvCache* cache, const DanceKvBatch* batch, uint32_t heads, uint32_t count) {
-  if (check_shapes(cache, batch) || heads == 0 || heads % cache->kv_heads || count == 0) return 0;
-  return (size_t)batch->tokens * cache->kv_heads * most_blocks(cache, batch) * 4;
+  if (check_shapes(cache, batch) || heads == 0 || heads % cache->kv_heads || count == 0 || batch->tokens == 0) return 0;
+  const SelectPlan p = select_plan(cache, batch, heads);
+  return p.fused ? 0 : (size_t)batch->tokens * cache->kv_heads * p.blocks * 4;
 }
 
 int dance_kv_select(const DanceKvCache* cache, const DanceKvBatch* batch, const DanceKvRows* queries, uint32_t count,
@@ -231,23 +488,32 @@ int dance_kv_select(const DanceKvCache* cache, const DanceKvBatch* batch, const 
     why = "count must be positive and hold sink and recent";
   if (why) KV_ERR("dance_kv_select", "%s", why);
   if (batch->tokens == 0) return 0;
+  const SelectPlan p = select_plan(cache, batch, queries->heads);
   const size_t need = dance_kv_select_work(cache, batch, queries->heads, count);
-  if (!work || work_bytes < need || !aligned(work, 16))
+  if (need && (!work || work_bytes < need || !aligned(work, 16)))
     KV_ERR("dance_kv_select", "work must hold %zu bytes, aligned to 16", need);
-  const uint32_t blocks = most_blocks(cache, batch);
+  const uint32_t per = kSelWaves * kTwo * 16u;
+  const uint32_t chunks = p.fused ? 1u : (p.blocks + per - 1) / per;
   const uint64_t units = (uint64_t)batch->tokens * cache->kv_heads;
-  const uint32_t per = 16 * kScoreWaves * 2;
-  const uint32_t chunks = (blocks + per - 1) / per;
-  if (units * chunks * 64 * kScoreWaves > 0xFFFFFFFFull || units * kTopThreads > 0xFFFFFFFFull)
+  if (p.groups * chunks * kSelThreads > 0xFFFFFFFFull || (!p.fused && units * kSelThreads > 0xFFFFFFFFull))
     KV_ERR("dance_kv_select", "batch is too large for one launch");
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const SelectArgs a{cache_args(cache), batch_args(batch), rows_args(queries), queries->heads / cache->kv_heads,
-                     count, sink, recent, blocks, static_cast<float*>(work), chosen};
+  const SelectArgs a{cache_args(cache), batch_args(batch), rows_args(queries), queries->heads / cache->kv_heads, p.gp,
+                     p.ntok, p.tiles, count, sink, recent, p.blocks, chunks, per, static_cast<uint32_t*>(work), chosen};
+  const bool vec = rows_vector(queries);
+  const size_t lds = (size_t)p.ntok * p.blocks * 4;
   with_kind(cache->dim, queries->dtype, [&](auto d, auto bf) {
-    hipLaunchKernelGGL((k_score<decltype(d)::value, decltype(bf)::value>), dim3((uint32_t)(units * chunks)),
-                       dim3(64 * kScoreWaves), 0, st, a, chunks, per);
+    auto go = [&](auto v) {
+      constexpr int D = decltype(d)::value;
+      constexpr bool BF = decltype(bf)::value, V = decltype(v)::value;
+      if (p.fused)
+        hipLaunchKernelGGL((k_select<D, BF, V>), dim3((uint32_t)p.groups), dim3(kSelThreads), lds, st, a);
+      else
+        hipLaunchKernelGGL((k_score<D, BF, V>), dim3((uint32_t)(p.groups * chunks)), dim3(kSelThreads), 0, st, a);
+    };
+    vec ? go(std::true_type{}) : go(std::false_type{});
   });
-  hipLaunchKernelGGL(k_top, dim3((uint32_t)units), dim3(kTopThreads), 0, st, a);
+  if (!p.fused) hipLaunchKernelGGL(k_top, dim3((uint32_t)units), dim3(kSelThreads), 0, st, a);
   return launched("dance_kv_select");
 }
 
