@@ -17,11 +17,13 @@
 // Codes go from memory to the registers that the MFMAs read; every code is
 // read once per 16 rows.
 //
-// Softmax: running reference M and sum l per row, in log2 units. A row keeps its M until
-// a logit exceeds it by 2^kSlack; weights are then at most 2^(kLift + kSlack), inside f16,
-// and the least normal weight is 2^-20 of a row's largest. The products take
-// weight * (value scale / largest value scale so far), which f16 rounds to 11
-// bits; the sum l takes the unrounded weights.
+// Softmax, in log2 units: with s a scaled logit and y its value's scale, the second
+// product takes p = 2^(s + log2 y - R), and the row's sum is l = sum p / y; the result is
+// the product over l. The logit's scale, log2 y and R make one fma of it. R is a running reference per
+// row that stays until s + log2 y exceeds it by kLift + kSlack: p is then at most
+// 2^(kLift + kSlack), inside f16, which rounds it to 11 bits (down to 2^-27 of a row's largest; the
+// f16 outputs have 11 bits too). l and all sums are float32, l of unrounded
+// p. Scales below 2^kLeastExp count as that, so that 1 / y is finite.
 
 #include <cfloat>
 #include <cmath>
@@ -46,7 +48,20 @@ constexpr uint32_t wide_waves(int d) { return d <= 192 ? 8 : 4; }
 // 9.6 + 3.8 us, 216 units of 3500 x 64 (448 KB) 16.6 and 13.8 + 3.9 us, 128 units of 4096 x
 // 128 (1 MB) 42.5 and 31.0 + 4.1 us.
 constexpr uint64_t kWideUnits = 256, kWideBytes = 512 << 10;
-constexpr float kLift = 6.f, kSlack = 8.f;
+// k_chunk from this many rows of a sequence and kv head on. Measured with k_step
+// and with k_chunk (bf16, 8 kv heads of 4, 128 dimensions): one sequence of 24 tokens over 8192
+// 26 and 39 us, of 256 over 2048 46 and 42, of 256 over 16384 217 and 114, of 4096 over 4096
+// 437 and 174 us; 32 of 8 tokens over 4000 84 and 133 us.
+constexpr uint64_t kChunkRows = 64;
+// Its workgroups have eight waves where that gives each CU two of them, else four:
+// 627 and 653 us for two chunks of 2048 tokens over 6000 to 10000, 42 and 36 us for
+// 1024 over 1024. Below one workgroup per CU the tokens are split, up to kChunkUnits workgroups
+// of at least kChunkSplitTiles tiles (64 tokens over 8192: 32 us at 8 tiles, 41 at 16).
+constexpr uint64_t kChunkSplitTiles = 8;
+constexpr uint64_t kChunkUnits = 512;
+constexpr int kChunkWide = 8, kChunkSmall = 4;
+constexpr float kLift = 13.f, kSlack = 2.f;
+constexpr float kLeastScale = 0x1p-100f;  // 2^kLeastExp
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kSplitUnits = 1024;  // workgroups that fill the chip several times over
 constexpr uint32_t kSplitTiles = 16;    // least tiles of a split: its partial sums are then 2 to 6 % of what it reads
@@ -61,13 +76,17 @@ struct StepArgs {
   uint32_t group, tiles, outer, splits, per;  // per: tiles of 64 tokens in a split
   uint16_t* __restrict__ out;
   float* __restrict__ lse;
-  float* __restrict__ part;  // splits > 1: [row][split][D] sums, then [row][split][2] (M, l)
+  float* __restrict__ part;  // splits > 1: [row][split][D] sums, then [row][split][2] (R, l)
 };
 
-// The work of one workgroup: 16 rows of one kv head, a split of the tokens they see.
-struct Unit {
-  uint32_t sq, h, tile, split;
-};
+// ln(l 2^R). R and the exponent of l are of opposite signs and about one size: their sum
+// first, or the logarithm's rounding is that of the larger number.
+__device__ __forceinline__ float lse_of(float R, float l) {
+  if (l == 0.f) return -__builtin_inff();
+  const uint32_t u = __float_as_uint(l);
+  const float e = (float)((int)(u >> 23) - 127), m = __uint_as_float((u & 0x7FFFFFu) | 0x3F800000u);
+  return l < __builtin_inff() ? ((R + e) + log2f(m)) * kLn2 : l;  // l is normal, infinite or NaN
+}
 
 template <int D, bool BF, bool LIST, bool VEC, uint32_t W>
 __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
@@ -134,7 +153,7 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
   f4_t acc[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) acc[t] = f4_t{0.f, 0.f, 0.f, 0.f};
-  float M = -FLT_MAX, l = 0.f, vref = 0.f, vinv = 0.f;
+  float R = -FLT_MAX, l = 0.f;
 
   // The block with the 16 tokens of group `grp` of a tile, and its first position; a hole: -1.
   auto locate = [&](uint32_t tt, uint32_t grp, int32_t& first) -> int32_t {
@@ -196,7 +215,7 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
     const size_t cell = (size_t)max(p.pv, 0) * a.c.kvh + h;
     const float2 x = *reinterpret_cast<const float2*>(a.c.scale + cell * 2);
     ks = p.pv >= 0 ? x.x : 0.f;
-    vs = p.pv >= 0 ? x.y : 0.f;
+    vs = p.pv >= 0 ? fmaxf(x.y, kLeastScale) : 1.f;
   };
 
   uint32_t tt = split * a.per + wave;
@@ -249,7 +268,7 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
   for (; tt < t_end; tt += W) {
     // tokens of this lane that its row sees: the first `lim` + 1 of its 16
     const int32_t lim = here.pv >= 0 && here.first <= pos ? pos - here.first : -1;
-    const float kq = ks * qscale, vcur = vs;
+    const float kq = ks * qscale, lv = __builtin_amdgcn_logf(vs), iv = 1.f / vs;
     const bool more = tt + W < t_end;
     f4_t sc[4];
 #pragma unroll
@@ -268,38 +287,32 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
     for (int st = 0; st < 4; ++st)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float x = sc[st][i] * kq;
-        sc[st][i] = 4 * st + i <= lim ? x : -__builtin_inff();
+        sc[st][i] = 4 * st + i <= lim ? __builtin_fmaf(sc[st][i], kq, lv) : -__builtin_inff();
         big = fmaxf(big, sc[st][i]);
       }
-    if (__any(big > M + (kLift + kSlack) || vcur > vref)) {
+    if (__any(big > R + (kLift + kSlack))) {
       // each row by its own logits alone: a row's result does not depend on its neighbours
       const float row_big = rows_max(big);
-      const float m_new = row_big > M + (kLift + kSlack) ? row_big - kLift : M;
-      const float v_new = fmaxf(vref, rows_max(vcur));
-      const float f = exp2f(M - m_new);
-      const float fo = v_new > 0.f ? f * (vref / v_new) : 0.f;
+      const float r_new = row_big > R + (kLift + kSlack) ? row_big - kLift : R;
+      const float f = exp2f(R - r_new);
       l *= f;
 #pragma unroll
       for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] *= fo;
-      M = m_new;
-      vref = v_new;
-      vinv = v_new > 0.f ? 1.f / v_new : 0.f;
+        for (int i = 0; i < 4; ++i) acc[t][i] *= f;
+      R = r_new;
     }
-    const float w = vcur * vinv;
     h8_t pf[2];
     float add = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float p = __builtin_amdgcn_exp2f(sc[2 * u + (i >> 2)][i & 3] - M);
+        const float p = __builtin_amdgcn_exp2f(sc[2 * u + (i >> 2)][i & 3] - R);
         add += p;
-        pf[u][i] = (_Float16)(p * w);
+        pf[u][i] = (_Float16)p;
       }
-    l += add;
+    l += add * iv;
 #pragma unroll
     for (int t = 0; t < DT; ++t) {
       acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vw[t].x, vw[t].y), pf[0], acc[t], 0, 0, 0);
@@ -315,13 +328,13 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
   // The waves' sums meet in LDS, in wave order.
   l = rows_sum(l);
   if (g == 0) {
-    sm_m[wave][n] = M;
+    sm_m[wave][n] = R;
     sm_l[wave][n] = l;
   }
 #pragma unroll
   for (int t = 0; t < DT; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sm_o[wave][n][16 * t + 4 * g + i] = acc[t][i] * vref;
+    for (int i = 0; i < 4; ++i) sm_o[wave][n][16 * t + 4 * g + i] = acc[t][i];
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < rows * (D / 4); i += 64 * W) {
     const uint32_t rr = i / (D / 4), d = i % (D / 4) * 4;
@@ -350,10 +363,12 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) y[x] = store_val<BF>(sum == 0.f ? 0.f : o[x] * inv);
       *reinterpret_cast<u2_t*>(a.out + row * D + d) = u2_t{y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16};
-      if (a.lse && d == 0) a.lse[row] = sum == 0.f ? -__builtin_inff() : (m + log2f(sum)) * kLn2;
+      if (a.lse && d == 0) a.lse[row] = lse_of(m, sum);
     }
   }
 }
+
+#include "kv_chunk.h"
 
 // Joins the splits of a row, one workgroup per row: the weights of up to 64
 // splits at a time in the lanes of every wave, the sums of the splits that have
@@ -383,15 +398,21 @@ __global__ __launch_bounds__(64 * (W == 1 ? kJoinRows : W)) void k_join(const fl
     const float f = l != 0.f ? exp2f(ml[2 * i] - m) : 0.f;  // a split without sums was not written
     total += f * l;
     const uint32_t n = min(64u, splits - i0);
-#pragma unroll
-    for (uint32_t k = wave * P; k < 64; k += W * P) {
-      const uint32_t mine = k + lane / L;
-      const float w = __shfl(f, (int)min(mine, 63u));
-      if (k < n && mine < n && lane < P * L) {
-        const f4_t x = *reinterpret_cast<const f4_t*>(po + (size_t)(i0 + mine) * D + lane % L * 4);
+    auto take = [&](uint32_t k) {
+      const uint32_t at = k + lane / L;
+      const float w = __shfl(f, (int)min(at, 63u));
+      if (at < n && lane < P * L) {
+        const f4_t x = *reinterpret_cast<const f4_t*>(po + (size_t)(i0 + at) * D + lane % L * 4);
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[c] += w != 0.f ? w * x[c] : 0.f;
       }
+    };
+    if constexpr (W == 1) {
+      for (uint32_t k = 0; k < n; k += P) take(k);
+    } else {
+#pragma unroll
+      for (uint32_t k = wave * P; k < 64; k += W * P)
+        if (k < n) take(k);
     }
   }
 #pragma unroll
@@ -412,14 +433,15 @@ __global__ __launch_bounds__(64 * (W == 1 ? kJoinRows : W)) void k_join(const fl
 #pragma unroll
     for (int c = 0; c < 4; ++c) z[c] = store_val<BF>(total == 0.f ? 0.f : y[c] * inv);
     *reinterpret_cast<u2_t*>(out + row * D + lane * 4) = u2_t{z[0] | (uint32_t)z[1] << 16, z[2] | (uint32_t)z[3] << 16};
-    if (lse && lane == 0) lse[row] = total == 0.f ? -__builtin_inff() : (m + log2f(total)) * kLn2;
+    if (lse && lane == 0) lse[row] = lse_of(m, total);
   }
 }
 
 struct Plan {
   uint64_t units;  // sequences or token rows, x row tiles x kv heads
   uint32_t tiles, splits, per;
-  bool wide;
+  bool wide, chunk;
+  int waves;  // of a workgroup of k_chunk
   size_t work;
 };
 Plan plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, bool list, uint32_t count) {
@@ -427,19 +449,27 @@ Plan plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, bool lis
   if (b->tokens == 0) return p;
   const uint64_t group = heads / c->kv_heads;
   const uint64_t rows = list ? group : group * b->max_tokens;
-  p.tiles = (uint32_t)((rows + kRowTile - 1) / kRowTile);
+  p.chunk = !list && rows > kChunkRows;
+  // by the rows that there are: sequences may have fewer than max_tokens
+  const uint64_t big = 32 * kChunkWide;
+  p.waves = c->dim <= 128 && (group * b->tokens + big - 1) / big * c->kv_heads >= kChunkUnits ? kChunkWide : kChunkSmall;
+  const uint32_t row_tile = p.chunk ? 32u * p.waves : kRowTile;
+  p.tiles = (uint32_t)((rows + row_tile - 1) / row_tile);
   p.units = (uint64_t)(list ? b->tokens : b->seqs) * p.tiles * c->kv_heads;
   // A split takes a fixed number of tiles, so that sequences of other lengths take
   // other numbers of workgroups.
   const uint64_t all = ((uint64_t)(list ? count : most_blocks(c, b)) * c->block_tokens + kTokTile - 1) / kTokTile;
-  p.wide = p.units <= kWideUnits && all * kTokTile * 2 * c->dim <= kWideBytes;
+  p.wide = !p.chunk && p.units <= kWideUnits && all * kTokTile * 2 * c->dim <= kWideBytes;
   if (p.wide) {
     p.per = (uint32_t)all;
     p.splits = 1;
     return p;
   }
-  uint64_t per = (p.units * all + kSplitUnits - 1) / kSplitUnits;
-  per = per < kSplitTiles ? kSplitTiles : (per + kStepWaves - 1) / kStepWaves * kStepWaves;
+  const uint64_t there = p.chunk ? (group * b->tokens + row_tile - 1) / row_tile * c->kv_heads : p.units;
+  const uint64_t want = p.chunk ? kChunkUnits : kSplitUnits, round = p.chunk ? 1 : kStepWaves;
+  uint64_t per = there * 2 >= want && p.chunk ? all : (there * all + want - 1) / want;
+  const uint64_t least = p.chunk ? kChunkSplitTiles : kSplitTiles;
+  per = per < least ? least : (per + round - 1) / round * round;
   p.per = (uint32_t)(per < all ? per : all);
   p.splits = (uint32_t)((all + p.per - 1) / p.per);
   if (p.splits > 1) p.work = (size_t)b->tokens * heads * p.splits * (c->dim + 2) * 4;
@@ -465,8 +495,10 @@ int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, c
     std::fprintf(stderr, "[%s] work must hold %zu bytes, aligned to 16\n", who, p.work);
     return -1;
   }
-  const uint64_t grid = p.units * p.splits;
-  if (grid * 64 * kStepWaves > 0xFFFFFFFFull || (uint64_t)batch->tokens * q->heads * 64 * kJoinWaves > 0xFFFFFFFFull) {
+  // k_chunk deals sequences and heads out eight at a time
+  const uint64_t pairs = (uint64_t)batch->seqs * cache->kv_heads;
+  const uint64_t grid = p.chunk && pairs > 8 ? (pairs + 7) / 8 * 8 * p.tiles * p.splits : p.units * p.splits;
+  if (grid * 64 * 8 > 0xFFFFFFFFull || (uint64_t)batch->tokens * q->heads * 64 * kJoinWaves > 0xFFFFFFFFull) {
     std::fprintf(stderr, "[%s] batch is too large for one launch\n", who);
     return -1;
   }
@@ -481,6 +513,18 @@ int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, c
     auto go = [&](auto l, auto v) {
       constexpr bool L = decltype(l)::value, V = decltype(v)::value;
       constexpr uint32_t W = wide_waves(D);
+      if constexpr (!L) {
+        if (p.chunk) {
+          if constexpr (D <= 128) {
+            if (p.waves == kChunkWide) {
+              hipLaunchKernelGGL((k_chunk<D, BF, V, kChunkWide>), dim3((uint32_t)grid), dim3(64 * kChunkWide), 0, st, a);
+              return;
+            }
+          }
+          hipLaunchKernelGGL((k_chunk<D, BF, V, kChunkSmall>), dim3((uint32_t)grid), dim3(64 * kChunkSmall), 0, st, a);
+          return;
+        }
+      }
       if (p.wide)
         hipLaunchKernelGGL((k_step<D, BF, L, V, W>), dim3((uint32_t)grid), dim3(64 * W), 0, st, a);
       else

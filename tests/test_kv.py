@@ -89,7 +89,7 @@ class Model:
         p = np.exp(x - m)
         lse = m + math.log(p.sum())
         p /= p.sum()
-        return p @ vals, lse, p @ np.abs(vals), float((np.abs(keys) @ np.abs(q)).max() * scale)
+        return p @ vals, lse, p @ np.abs(vals), float((np.abs(keys) @ np.abs(q)).max() * abs(scale))
 
     def attention(self, q, table, lengths, offsets, scale, lists=None):
         t, heads, dim = q.shape
@@ -183,7 +183,8 @@ def numbers(t):
 def check_attention(model, got, lse, q, table, lens, off, scale, lists=None):
     o, l, absolute, g = model.attention(numbers(q), table, lens, off, scale, lists)
     d = g * (model.dim + 8) * 2.0 ** -24
-    o = np.where(np.abs(o) < LEAST[q.dtype] / 2, 0.0, o)  # what the output's type cannot tell from zero
+    least = LEAST[q.dtype]  # subnormal values are those that the output's type has
+    o = np.where(np.abs(o) < least / ROUND[q.dtype], np.rint(o / least) * least, o)
     tol = ROUND[q.dtype] * np.abs(o) + (2.0 ** -11 + 2 * d[..., None] + 2.0 ** -18) * absolute
     err = np.abs(numbers(got) - o)
     assert (err <= tol).all(), (float((err - tol).max()), np.unravel_index((err - tol).argmax(), err.shape))
@@ -224,6 +225,33 @@ def test_attention(shape, holes):
     got, lse = kv.attention(cache, q, dev(table), dev(np.int32(lens)), dev(off) if news else None, return_lse=True,
                             max_tokens=max(news) if news else None)
     check_attention(Model(cache), got, lse, q, table, lens, off, dim ** -0.5)
+
+
+# many rows of a sequence: prompts, their chunks, with earlier tokens and without
+PROMPTS = [
+    (1, 4, 128, 64, BF16, [200, 333, 0, 64], [200, 70, 3, 64]),
+    (2, 3, 96, 32, F16, [257, 31, 1], [257, 31, 1]),
+    (1, 2, 192, 16, BF16, [150, 65], [130, 65]),
+    (1, 1, 256, 128, F16, [129, 400], [129, 90]),
+    (3, 1, 64, 16, BF16, [300, 20, 90], [100, 33, 90]),
+    (1, 24, 128, 32, F16, [70, 9], [20, 12]),      # rows before the first token
+    (1, 2, 64, 64, BF16, [5000, 4100], [40, 60]),  # few rows over many tokens: split
+    (9, 2, 64, 32, BF16, [64, 130, 70], [64, 40, 70]),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", PROMPTS, ids=[f"{s[0]}x{s[1]}-{s[2]}-{s[3]}-{str(s[4])[6:]}" for s in PROMPTS])
+@pytest.mark.parametrize("holes,scale", [(0, None), (3, 0.3), (0, -0.1), (0, 0.0)])
+def test_attention_of_prompts(shape, holes, scale):
+    heads, group, dim, bs, dt, lens, news = shape
+    rng = np.random.default_rng(17)
+    cache, table = make(rng, heads, dim, bs, lens, holes, pow2=scale is None)
+    off = offsets_of(news)
+    q = torch.from_numpy(rng.normal(size=(off[-1], heads * group, dim))).to(dt).cuda()
+    got, lse = kv.attention(cache, q, dev(table), dev(np.int32(lens)), dev(off), scale=scale, return_lse=True,
+                            max_tokens=max(news))
+    check_attention(Model(cache), got, lse, q, table, lens, off, dim ** -0.5 if scale is None else scale)
 
 
 @pytest.mark.gpu
