@@ -93,7 +93,8 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
   constexpr int KS = D / 32;  // inner steps of the first product
   constexpr int DT = D / 16;  // row tiles of the second
   constexpr int KW = D / 16;  // words of a key row that a lane holds
-  __shared__ float sm_o[W][kRowTile][D];
+  // rows 16 bytes longer than their values: 16 of them lie in different banks
+  __shared__ __attribute__((aligned(16))) float sm_o[W][kRowTile][D + 4];
   __shared__ float sm_m[W][kRowTile], sm_l[W][kRowTile];
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const uint32_t n = lane & 15u, g = lane >> 4;
@@ -331,27 +332,28 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
     sm_m[wave][n] = R;
     sm_l[wave][n] = l;
   }
+  if (n < rows)
 #pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sm_o[wave][n][16 * t + 4 * g + i] = acc[t][i];
+    for (int t = 0; t < DT; ++t) *reinterpret_cast<f4_t*>(&sm_o[wave][n][16 * t + 4 * g]) = acc[t];
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < rows * (D / 4); i += 64 * W) {
     const uint32_t rr = i / (D / 4), d = i % (D / 4) * 4;
     float m = sm_m[0][rr];
 #pragma unroll
     for (uint32_t w = 1; w < W; ++w) m = fmaxf(m, sm_m[w][rr]);
-    float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+    f4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (uint32_t w = 0; w < W; ++w) {
       const float f = exp2f(sm_m[w][rr] - m);
       sum += f * sm_l[w][rr];
+      const f4_t y = *reinterpret_cast<const f4_t*>(&sm_o[w][rr][d]);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) o[x] += f * sm_o[w][rr][d + x];
+      for (int x = 0; x < 4; ++x) o[x] += f * y[x];
     }
     const size_t row = row_of(rr);
     if (a.splits > 1) {
-      *reinterpret_cast<f4_t*>(a.part + (row * a.splits + split) * D + d) = f4_t{o[0], o[1], o[2], o[3]};
+      *reinterpret_cast<f4_t*>(a.part + (row * a.splits + split) * D + d) = o;
       if (d == 0) {
         float* const pm = part_ml + (row * a.splits + split) * 2;
         pm[0] = m;

@@ -53,6 +53,12 @@ class DanceKvRows(C.Structure):
 
 
 _bound = None
+# torch's handle of the current stream, without the Stream object around it where torch has that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(index):
+    return _raw_stream(index) if _raw_stream else torch.cuda.current_stream(index).cuda_stream
 
 
 def _bind():
@@ -168,12 +174,12 @@ def _batch(cache, rows, table, lengths, offsets, max_tokens, max_length):
 
 
 def _call(name, cache, *args):
-    fn = getattr(_bind(), name)
-    if torch.cuda.current_device() != cache.device.index:
-        with torch.cuda.device(cache.device):
-            rc = fn(cache._ref, *args, torch.cuda.current_stream().cuda_stream)
+    fn, index = getattr(_bound, name), cache.device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            rc = fn(cache._ref, *args, _stream(index))
     else:
-        rc = fn(cache._ref, *args, torch.cuda.current_stream().cuda_stream)
+        rc = fn(cache._ref, *args, _stream(index))
     if rc != 0:
         raise RuntimeError(f"{name} failed with return code {rc}")
 
@@ -200,6 +206,7 @@ def append(cache, k, v, table, lengths, offsets=None, max_tokens=None):
     if k.shape != v.shape or k.dtype != v.dtype:
         raise ValueError("k and v must have one shape and type")
     b = _batch(cache, k, table, lengths, offsets, max_tokens, None)
+    _bind()
     if k.shape[0]:
         _call("dance_kv_append", cache, C.byref(b), C.byref(kr), C.byref(vr))
 
