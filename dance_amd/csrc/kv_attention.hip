@@ -13,7 +13,8 @@
 //  - those registers are, in their order, the weights' operand of the second
 //    product, whose value operand is then 16 adjacent bytes of a dimension's
 //    tokens: one load, as values lie dims-major;
-//  - lane group g holds dimensions g D / 4 .. of keys and queries, adjacent bytes too.
+//  - of keys and queries lane group g holds every fourth piece of 16 dimensions (8
+//    where dim is no multiple of 64): a load then takes 64 adjacent bytes of a token.
 // Codes go from memory to the registers that the MFMAs read; every code is
 // read once per 16 rows.
 //
@@ -42,12 +43,12 @@ constexpr uint32_t kRowTile = 16;
 constexpr uint32_t kTokTile = 64;
 // Waves of a workgroup that takes all of a row tile's tokens: what the registers allow.
 constexpr uint32_t wide_waves(int d) { return d <= 192 ? 8 : 4; }
-// It needs no join, but leaves CUs idle and their bandwidth unused: up to one
-// workgroup per CU, up to so many bytes of codes for each. Measured with it and
-// with splits (and their join): 8 units of 704 tokens of 128 dimensions 10.5 and
-// 9.6 + 3.8 us, 216 units of 3500 x 64 (448 KB) 16.6 and 13.8 + 3.9 us, 128 units of 4096 x
-// 128 (1 MB) 42.5 and 31.0 + 4.1 us.
-constexpr uint64_t kWideUnits = 256, kWideBytes = 512 << 10;
+// It needs no join (and its launch), but a CU reads 75 GB/s at most: up to one
+// workgroup per CU and kWideBytes of codes for each, more where many keep the chip
+// busy anyway. Measured with it and with splits, of 128 dimensions (whole calls): 8 units of 1024
+// tokens 11.6 and 13.5 us, of 2048 16.7 and 14.1 us; kernels alone: 216 units of 3500 x 64
+// (448 KB) 16.0 and 13.8 + 3.9 us, 128 of 4096 x 128 (1 MB) 42.5 and 31.0 + 4.1 us.
+constexpr uint64_t kWideUnits = 256, kWideBytes = 256 << 10;
 // k_chunk from this many rows of a sequence and kv head on. Measured with k_step
 // and with k_chunk (bf16, 8 kv heads of 4, 128 dimensions): one sequence of 24 tokens over 8192
 // 26 and 39 us, of 256 over 2048 46 and 42, of 256 over 16384 217 and 114, of 4096 over 4096
@@ -93,6 +94,7 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
   constexpr int KS = D / 32;  // inner steps of the first product
   constexpr int DT = D / 16;  // row tiles of the second
   constexpr int KW = D / 16;  // words of a key row that a lane holds
+  constexpr int kPiece = KW % 4 == 0 ? 16 : 8;
   // rows 16 bytes longer than their values: 16 of them lie in different banks
   __shared__ __attribute__((aligned(16))) float sm_o[W][kRowTile][D + 4];
   __shared__ float sm_m[W][kRowTile], sm_l[W][kRowTile];
@@ -187,19 +189,19 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
   auto load_keys = [&](uint32_t tt, const Place& p) {
     const uint32_t slot = (tt * kTokTile + (n >> 2) * 16u) & (bs - 1u);
     const size_t cell = (size_t)max(p.pk, 0) * a.c.kvh + h;
-    const int8_t* const kp = a.c.k + ((cell << bsh) + slot + (n & 3u)) * D + g * (D / 4);
+    const int8_t* const kp = a.c.k + ((cell << bsh) + slot + (n & 3u)) * D + g * kPiece;
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
       if constexpr (KW % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < KW / 4; ++i) {
-          const u4_t w = *reinterpret_cast<const u4_t*>(kp + (size_t)st * 4 * D + i * 16);
+          const u4_t w = *reinterpret_cast<const u4_t*>(kp + (size_t)st * 4 * D + i * 64);
           kw[st][4 * i] = w.x, kw[st][4 * i + 1] = w.y, kw[st][4 * i + 2] = w.z, kw[st][4 * i + 3] = w.w;
         }
       } else {
 #pragma unroll
         for (int i = 0; i < KW / 2; ++i) {
-          const u2_t w = *reinterpret_cast<const u2_t*>(kp + (size_t)st * 4 * D + i * 8);
+          const u2_t w = *reinterpret_cast<const u2_t*>(kp + (size_t)st * 4 * D + i * 32);
           kw[st][2 * i] = w.x, kw[st][2 * i + 1] = w.y;
         }
       }
@@ -225,14 +227,15 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
   if (any) here = place(tt);
   u4_t raw[KS];
   {
-    const uint16_t* src = a.q.data + (int64_t)(s.row + tok) * a.q.token_stride + (int64_t)head * a.q.head_stride + g * (D / 4);
+    const uint16_t* src = a.q.data + (int64_t)(s.row + tok) * a.q.token_stride + (int64_t)head * a.q.head_stride + g * kPiece;
 #pragma unroll
     for (int c = 0; c < KS; ++c) {
+      const uint16_t* const at = src + (kPiece == 16 ? 64 * (c / 2) + 8 * (c % 2) : 32 * c);
       if constexpr (VEC) {
-        raw[c] = *reinterpret_cast<const u4_t*>(src + 8 * c);
+        raw[c] = *reinterpret_cast<const u4_t*>(at);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) raw[c][i] = (uint32_t)src[8 * c + 2 * i] | (uint32_t)src[8 * c + 2 * i + 1] << 16;
+        for (int i = 0; i < 4; ++i) raw[c][i] = (uint32_t)at[2 * i] | (uint32_t)at[2 * i + 1] << 16;
       }
     }
   }
@@ -461,7 +464,7 @@ Plan plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, bool lis
   // A split takes a fixed number of tiles, so that sequences of other lengths take
   // other numbers of workgroups.
   const uint64_t all = ((uint64_t)(list ? count : most_blocks(c, b)) * c->block_tokens + kTokTile - 1) / kTokTile;
-  p.wide = !p.chunk && p.units <= kWideUnits && all * kTokTile * 2 * c->dim <= kWideBytes;
+  p.wide = !p.chunk && p.units <= kWideUnits && all * kTokTile * 2 * c->dim <= kWideBytes + (p.units << 10);
   if (p.wide) {
     p.per = (uint32_t)all;
     p.splits = 1;

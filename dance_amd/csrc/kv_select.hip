@@ -26,9 +26,8 @@ namespace dance {
 namespace kv {
 namespace {
 
-constexpr uint32_t kSelWaves = 8;
+constexpr uint32_t kSelWaves = 16;
 constexpr uint32_t kSelThreads = 64 * kSelWaves;
-constexpr uint32_t kTwo = 2;  // block tiles of 16 that a wave has on the way at once
 
 constexpr uint32_t kNoKey = 0x007FFFFFu;   // of -inf: holes
 constexpr uint32_t kForced = 0xFFFFFFFFu;  // above all scores
@@ -74,6 +73,7 @@ struct Codes {
   static constexpr uint32_t kStride = 2 * D + 16;
   int8_t c[kRowTiles * 16 * kStride];
   float up[kRowTiles * 16];  // 2^e of a row's codes; 0: no row
+  uint32_t seen[kRowTiles * 16];  // blocks that a token row sees
 };
 
 // Codes of row tiles [p0, p0 + kRowTiles): a wave's four lane groups of 16 take a row each.
@@ -119,54 +119,102 @@ __device__ __forceinline__ void code_rows(const SelectArgs& a, const Tokens& tk,
   }
 }
 
+// Between the lanes that differ in bit X (1 or 2): the lower one gives its y for the other's x.
+template <int X>
+__device__ __forceinline__ void swap_pieces(i4_t& x, i4_t& y, bool upper) {
+  constexpr int perm = X == 1 ? 0xB1 : 0x4E;  // quad lanes 1 0 3 2, 2 3 0 1
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int got = __builtin_amdgcn_mov_dpp(upper ? x[w] : y[w], perm, 0xF, 0xF, true);
+    x[w] = upper ? got : x[w];
+    y[w] = upper ? y[w] : got;
+  }
+}
+
 // Keys of blocks [from, to) for the workgroup's token rows: keys[t * stride + block].
 template <int D, bool BF, bool VEC>
 __device__ __forceinline__ void score_blocks(const SelectArgs& a, const Tokens& tk, uint32_t h, uint32_t from,
                                              uint32_t to, uint32_t* __restrict__ keys, size_t stride, Codes<D>& qc) {
   constexpr int KS = D / 32;  // inner steps of 64 over 2 D
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t n = lane & 15u, g = lane >> 4;
   const int32_t* const table = a.b.table + (size_t)tk.sq * a.b.width;
   const uint32_t per_tile = 16u / a.gp;  // token rows of a row tile
   const uint32_t rows = a.group > 16u ? (a.group + 15u) / 16u : (tk.n + per_tile - 1u) / per_tile;
+  for (uint32_t t = threadIdx.x; t < tk.n; t += kSelThreads) qc.seen[t] = tk.seen(a, t);
+  // A wave takes adjacent tiles of 16 blocks, four at a time: their places come with one
+  // load, their scales with another. The bounds of two tiles (of one, beyond 128 dimensions: registers)
+  // are on their way while a third is computed.
+  constexpr bool kDeep = D <= 128;
+  struct Tile {
+    i4_t b[KS];
+  };
+  const uint32_t all = (to - from + 15u) / 16u, share = (all + kSelWaves - 1) / kSelWaves;
+  const uint32_t t_end = min(all, (wave + 1) * share), t_begin = min(t_end, wave * share);
+  struct Four {  // lane i: block i of the 64
+    int32_t ph;
+    float ks;
+  };
+  auto places = [&](uint32_t tile) {
+    const uint32_t blk = from + tile * 16u + lane;
+    const int32_t ph = blk < to && tile < t_end ? table[blk] : -1;
+    Four f{(uint32_t)ph < a.c.blocks ? ph : -1, 0.f};
+    if (f.ph >= 0) f.ks = a.c.scale[((size_t)f.ph * a.c.kvh + h) * 2];
+    return f;
+  };
+  // A load instruction that takes 16 bytes of each of 16 blocks costs the address unit a
+  // turn for each of its 64 lanes (37 GB/s a CU). So S neighbouring lanes take S
+  // adjacent pieces of one block, S loads the blocks of S lanes, and turned() exchanges
+  // them: lane r of the S gets all pieces of block r.
+  constexpr int S = KS % 4 == 0 ? 4 : KS % 2 == 0 ? 2 : 1;
+  auto load = [&](const Four& f, uint32_t i) {
+    Tile t;
+#pragma unroll
+    for (int c = 0; c < S; ++c) {
+      const int32_t ph = __shfl(f.ph, (int)(16u * i + (n & ~(uint32_t)(S - 1)) + c));
+      const int8_t* const bp = a.c.bound + ((size_t)max(ph, 0) * a.c.kvh + h) * 2 * D + (g * S + (n & (S - 1))) * 16;
+#pragma unroll
+      for (int k = 0; k < KS / S; ++k) t.b[k * S + c] = *reinterpret_cast<const i4_t*>(bp + k * S * 64);
+    }
+    return t;
+  };
+  auto turned = [&](Tile& t) {
+    if constexpr (S > 1) {
+#pragma unroll
+      for (int k = 0; k < KS; k += S) {
+#pragma unroll
+        for (int c = 0; c < S; c += 2) swap_pieces<1>(t.b[k + c], t.b[k + c + 1], n & 1u);
+        if constexpr (S == 4) {
+          swap_pieces<2>(t.b[k], t.b[k + 2], n & 2u);
+          swap_pieces<2>(t.b[k + 1], t.b[k + 3], n & 2u);
+        }
+      }
+    }
+  };
+  // where in a row of 2 D codes the inner step c of this lane group stands
+  auto piece = [&](int c) { return (uint32_t)(c / S * S * 64 + c % S * 16) + g * S * 16u; };
+  Four four = places(t_begin);
   for (uint32_t p0 = 0; p0 < rows; p0 += kRowTiles) {
     if (p0) __syncthreads();
     code_rows<D, BF, VEC>(a, tk, h, p0, rows, qc);
     __syncthreads();
     const uint32_t here = min((uint32_t)kRowTiles, rows - p0);
-    struct Tile {
-      i4_t b[KS];
-      int32_t ph;
-      float ks;
-    };
-    auto load = [&](uint32_t blk) {
-      Tile t;
-      t.ph = blk < to ? table[blk] : -1;
-      if ((uint32_t)t.ph >= a.c.blocks) t.ph = -1;
-      const size_t cell = (size_t)max(t.ph, 0) * a.c.kvh + h;
-      const int8_t* const bp = a.c.bound + cell * 2 * D + g * (D / 2);
-#pragma unroll
-      for (int c = 0; c < KS; ++c) t.b[c] = *reinterpret_cast<const i4_t*>(bp + 16 * c);
-      t.ks = a.c.scale[cell * 2];
-      return t;
-    };
     auto put = [&](uint32_t t, uint32_t blk, bool hole, float x, bool add) {
       if (t >= tk.n || blk >= to) return;
-      const uint32_t seen = tk.seen(a, t);
+      const uint32_t seen = qc.seen[t];
       uint32_t key = sort_key(x + 0.f);
       if (blk < a.sink || blk + a.recent >= seen) key = kForced;
       if (hole) key = kNoKey;
       uint32_t* const at = keys + t * stride + blk;
       *at = add ? max(key, *at) : key;  // more than 16 heads: the same lane's key of those before
     };
-    auto score = [&](const Tile& b, uint32_t blk, uint32_t r, const i4_t* qf, const float* up) {
+    auto score = [&](const Tile& b, float ks, bool hole, uint32_t blk, uint32_t r, const i4_t* qf, const float* up) {
       i4_t acc = {0, 0, 0, 0};
 #pragma unroll
       for (int c = 0; c < KS; ++c) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf[c], b.b[c], acc, 0, 0, 0);
       float x[4];  // rows 4 g + i of block n
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = up[i] > 0.f ? ((float)acc[i] * b.ks) * up[i] : -__builtin_inff();
-      const bool hole = b.ph < 0;
+      for (int i = 0; i < 4; ++i) x[i] = up[i] > 0.f ? ((float)acc[i] * ks) * up[i] : -__builtin_inff();
       const uint32_t t0 = (p0 + r) * per_tile;
       if (a.group > 16u) {
         const float m = rows_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
@@ -190,47 +238,60 @@ __device__ __forceinline__ void score_blocks(const SelectArgs& a, const Tokens& 
         }
       }
     };
-    constexpr uint32_t kStep = kSelWaves * kTwo * 16u;
-    Tile cur[kTwo];
-    uint32_t blk = from + wave * kTwo * 16u + n;
-    if (blk - n < to)
+    if (p0) four = places(t_begin);
+    Tile t0 = load(four, 0), t1;
+    if constexpr (kDeep) t1 = load(four, 1);
+    for (uint32_t tile = t_begin; tile < t_end; tile += 4) {
+      const Four next = places(tile + 4);
 #pragma unroll
-      for (uint32_t u = 0; u < kTwo; ++u) cur[u] = load(blk + 16u * u);
-    for (; blk - n < to; blk += kStep) {
-      Tile nxt[kTwo];
-      const bool more = blk - n + kStep < to;
-      if (more)
+      for (uint32_t i = 0; i < 4; ++i) {
+        if (tile + i >= t_end) break;
+        constexpr uint32_t kAhead = kDeep ? 2 : 1;
+        Tile t2;
+        if (tile + i + kAhead < t_end) t2 = i + kAhead < 4 ? load(four, i + kAhead) : load(next, i + kAhead - 4);
+        const bool hole = __shfl(four.ph, (int)(16u * i + n)) < 0;
+        const float ks = __shfl(four.ks, (int)(16u * i + n));
+        turned(t0);
+        for (uint32_t r = 0; r < here; ++r) {
+          i4_t qf[KS];
+          float up[4];
 #pragma unroll
-        for (uint32_t u = 0; u < kTwo; ++u) nxt[u] = load(blk + kStep + 16u * u);
-      for (uint32_t r = 0; r < here; ++r) {
-        i4_t qf[KS];
-        float up[4];
+          for (int c = 0; c < KS; ++c)
+            qf[c] = *reinterpret_cast<const i4_t*>(qc.c + (r * 16u + n) * Codes<D>::kStride + piece(c));
 #pragma unroll
-        for (int c = 0; c < KS; ++c)
-          qf[c] = *reinterpret_cast<const i4_t*>(qc.c + (r * 16u + n) * Codes<D>::kStride + g * (D / 2) + 16 * c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) up[i] = qc.up[r * 16u + 4 * g + i];
-#pragma unroll
-        for (uint32_t u = 0; u < kTwo; ++u) score(cur[u], blk + 16u * u, r, qf, up);
+          for (int x = 0; x < 4; ++x) up[x] = qc.up[r * 16u + 4 * g + x];
+          score(t0, ks, hole, from + (tile + i) * 16u + n, r, qf, up);
+        }
+        if constexpr (kDeep) {
+          t0 = t1;
+          t1 = t2;
+        } else {
+          t0 = t2;
+        }
       }
-      if (more)
-#pragma unroll
-        for (uint32_t u = 0; u < kTwo; ++u) cur[u] = nxt[u];
+      four = next;
     }
   }
 }
 
-// What a team of W waves shares while it chooses.
+// What a team of W waves shares while it chooses. A team of one wave clears its
+// counters itself; a team of several has a cleared set for each of the four
+// rounds (clear_teams), and every wave reads them, so that a round takes one barrier.
 struct Team {
   uint32_t hist[256];
-  uint32_t lo, hi, digit, left;          // W > 1
-  uint32_t more[kSelWaves], same[kSelWaves], forced[kSelWaves];
 };
+struct Shared {  // W > 1: each wave's
+  uint32_t lo[kSelWaves], hi[kSelWaves], some[kSelWaves], forced[kSelWaves], more[kSelWaves], same[kSelWaves];
+};
+constexpr int kRounds = 4;  // of 8 bits
+__device__ __forceinline__ void clear_teams(Team* tm) {
+  for (uint32_t i = threadIdx.x; i < kRounds * 256; i += kSelThreads) tm[i >> 8].hist[i & 255u] = 0;
+}
 
 // The `count` blocks of the n with the largest keys, ties to the lower block, ascending.
 template <uint32_t W>
 __device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32_t n, uint32_t count,
-                                       int32_t* __restrict__ out, Team& tm) {
+                                       int32_t* __restrict__ out, Team* tm, Shared& sh) {
   const uint32_t lane = threadIdx.x & 63u, wave = W == 1 ? 0u : threadIdx.x >> 6;
   const uint32_t tid = W == 1 ? lane : threadIdx.x;
   auto sync = [&] {
@@ -244,33 +305,32 @@ __device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32
   };
   // Range of the keys that compete, how many they are, and how many are forced.
   uint32_t lo = ~0u, hi = 0, some = 0, forced = 0;
+#pragma unroll 4
   for (uint32_t i = tid; i < n; i += 64 * W) {
     const uint32_t k = keys[i];
-    if (k == kForced) {
-      ++forced;
-    } else if (k > kNoKey) {
-      lo = min(lo, k);
-      hi = max(hi, k);
-      ++some;
+    const bool f = k == kForced, in = k > kNoKey && !f;
+    forced += f;
+    some += in;
+    lo = min(lo, in ? k : ~0u);
+    hi = max(hi, in ? k : 0u);
+  }
+  auto reduce = [&](uint32_t lanes) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      if ((uint32_t)d >= lanes) break;
+      lo = min(lo, (uint32_t)__shfl_xor((int)lo, d));
+      hi = max(hi, (uint32_t)__shfl_xor((int)hi, d));
+      some += (uint32_t)__shfl_xor((int)some, d);
+      forced += (uint32_t)__shfl_xor((int)forced, d);
     }
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    lo = min(lo, (uint32_t)__shfl_xor((int)lo, d));
-    hi = max(hi, (uint32_t)__shfl_xor((int)hi, d));
-    some += (uint32_t)__shfl_xor((int)some, d);
-    forced += (uint32_t)__shfl_xor((int)forced, d);
-  }
+  };
+  reduce(64);
   if constexpr (W > 1) {
-    if (tid == 0) tm.lo = ~0u, tm.hi = 0;
-    if (lane == 0) tm.more[wave] = some, tm.forced[wave] = forced;
+    if (lane == 0) sh.lo[wave] = lo, sh.hi[wave] = hi, sh.some[wave] = some, sh.forced[wave] = forced;
     __syncthreads();
-    if (lane == 0) atomicMin(&tm.lo, lo), atomicMax(&tm.hi, hi);
-    some = forced = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < W; ++w) some += tm.more[w], forced += tm.forced[w];
-    __syncthreads();
-    lo = tm.lo, hi = tm.hi;
+    const uint32_t w = lane & (W - 1u);
+    lo = sh.lo[w], hi = sh.hi[w], some = sh.some[w], forced = sh.forced[w];
+    reduce(W);
   }
   // All keys above `limit` are taken, and the first `ties` equal to it.
   uint32_t want = less(count, forced), limit, ties = 0;
@@ -279,49 +339,43 @@ __device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32
   } else if (want == 0) {
     limit = kForced - 1u;
   } else {
-    while (true) {
+    for (int round = 0;; ++round) {  // ends: a round of four at most has shift 0
       const uint32_t bits = 32u - (uint32_t)__clz((int)(hi - lo | 1u));
       const uint32_t shift = less(bits, 8u);
-      for (uint32_t i = tid; i < 256; i += 64 * W) tm.hist[i] = 0;
-      sync();
+      uint32_t* const hist = tm[W == 1 ? 0 : round].hist;
+      if constexpr (W == 1) {
+        for (uint32_t i = tid; i < 256; i += 64) hist[i] = 0;
+        sync();
+      }
+#pragma unroll 4
       for (uint32_t i = tid; i < n; i += 64 * W) {
         const uint32_t k = keys[i];
-        if (k >= lo && k <= hi) atomicAdd(&tm.hist[(k - lo) >> shift], 1u);
+        if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> shift], 1u);
       }
       sync();
-      uint32_t digit = 0, left = 0;
-      if (W == 1 || wave == 0) {
-        // lane i has counters 4 i .. 4 i + 3; counted from the largest down
-        uint32_t c[4], mine = 0;
+      // lane i has counters 4 i .. 4 i + 3; counted from the largest down
+      uint32_t c[4], mine = 0;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) c[x] = tm.hist[4 * lane + x], mine += c[x];
-        uint32_t from = mine;  // over this lane and those after it
+      for (int x = 0; x < 4; ++x) c[x] = hist[4 * lane + x], mine += c[x];
+      uint32_t from = mine;  // over this lane and those after it
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const uint32_t o = (uint32_t)__shfl_down((int)from, d);
-          if (lane + d < 64) from += o;
-        }
-        uint32_t above = from - mine;
-        const bool here = above < want && from >= want;
-        uint32_t dg = 0, rest = 0, full = 0;
-#pragma unroll
-        for (int x = 3; x >= 0; --x) {
-          if (above < want && above + c[x] >= want) dg = 4 * lane + x, rest = want - above, full = c[x] == rest;
-          above += c[x];
-        }
-        const int src = __ffsll((unsigned long long)__ballot(here)) - 1;
-        digit = (uint32_t)__shfl((int)dg, src);
-        left = (uint32_t)__shfl((int)rest, src) | (uint32_t)__shfl((int)full, src) << 31;
+      for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = (uint32_t)__shfl_down((int)from, d);
+        if (lane + d < 64) from += o;
       }
-      if constexpr (W > 1) {
-        if (tid == 0) tm.digit = digit, tm.left = left;
-        __syncthreads();
-        digit = tm.digit, left = tm.left;
-        __syncthreads();
+      uint32_t above = from - mine;
+      const bool here = above < want && from >= want;
+      uint32_t digit = 0, left = 0, full = 0;
+#pragma unroll
+      for (int x = 3; x >= 0; --x) {
+        if (above < want && above + c[x] >= want) digit = 4 * lane + x, left = want - above, full = c[x] == left;
+        above += c[x];
       }
+      const int src = __ffsll((unsigned long long)__ballot(here)) - 1;
+      digit = (uint32_t)__shfl((int)digit, src);
+      want = (uint32_t)__shfl((int)left, src);
       lo += digit << shift;
-      want = left & 0x7FFFFFFFu;
-      if (left >> 31) {  // all of this counter's keys
+      if (__shfl((int)full, src)) {  // all of this counter's keys
         limit = lo - 1u;
         break;
       }
@@ -331,14 +385,16 @@ __device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32
         break;
       }
       hi = lo + min(hi - lo, (1u << shift) - 1u);
+      if constexpr (W == 1) sync();
     }
   }
   // Each wave takes its part of the blocks, in order.
   const uint32_t part = ((n + W - 1) / W + 63u) & ~63u;
   const uint32_t b0 = min(n, wave * part), b1 = min(n, b0 + part);
-  uint32_t at = 0, rank = 0;
+  uint32_t first = 0, rank = 0, total = 0, ranks = 0;  // taken, and equal to the limit, before this part and in all
   if constexpr (W > 1) {
     uint32_t more = 0, same = 0;
+#pragma unroll 4
     for (uint32_t i = b0 + lane; i < b1; i += 64) {
       const uint32_t k = keys[i];
       more += k > limit;
@@ -346,12 +402,16 @@ __device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) more += (uint32_t)__shfl_xor((int)more, d), same += (uint32_t)__shfl_xor((int)same, d);
-    if (lane == 0) tm.more[wave] = more, tm.same[wave] = same;
+    if (lane == 0) sh.more[wave] = more, sh.same[wave] = same;
     __syncthreads();
 #pragma unroll
-    for (uint32_t w = 0; w < W; ++w)
-      if (w < wave) at += tm.more[w] + min(tm.same[w], less(ties, rank)), rank += tm.same[w];
+    for (uint32_t w = 0; w < W; ++w) {
+      if (w == wave) first = total, rank = ranks;
+      total += sh.more[w] + min(sh.same[w], less(ties, ranks));
+      ranks += sh.same[w];
+    }
   }
+  uint32_t at = first;
   const uint64_t below = (1ull << lane) - 1;
   for (uint32_t i0 = b0; i0 < b1; i0 += 64) {
     const uint32_t i = i0 + lane;
@@ -366,15 +426,20 @@ __device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32
     at += (uint32_t)__popcll(got);
   }
   // -1 behind them
-  uint32_t total = at;
-  if constexpr (W > 1) {
-    __syncthreads();
-    if (wave == W - 1 && lane == 0) tm.lo = at;
-    __syncthreads();
-    total = tm.lo;
-  }
+  if constexpr (W == 1) total = at;
   for (uint32_t i = total + tid; i < count; i += 64 * W) out[i] = -1;
-  sync();
+  if constexpr (W == 1) sync();
+}
+
+// A workgroup's head and its index over the rest: all heads of eight such indexes
+// in turn, so that the heads of a block, whose bounds and scales share lines and
+// pages, are read by one XCD (workgroups go round the eight).
+struct Work {
+  uint32_t h, rest;
+};
+__device__ __forceinline__ Work work_of(uint32_t kvh) {
+  const uint32_t id = blockIdx.x;
+  return Work{id / 8u % kvh, id / 8u / kvh * 8u + id % 8u};
 }
 
 // Scores in LDS, chosen by the workgroup that made them.
@@ -382,22 +447,24 @@ template <int D, bool BF, bool VEC>
 __global__ __launch_bounds__(kSelThreads) void k_select(SelectArgs a) {
   extern __shared__ uint32_t lds_keys[];
   __shared__ Team teams[kSelWaves];
+  __shared__ Shared shared;
   __shared__ __attribute__((aligned(16))) Codes<D> codes;
-  uint32_t id = blockIdx.x;
-  const uint32_t h = id % a.c.kvh;
-  id /= a.c.kvh;
-  const Tokens tk = tokens_of(a, id / a.tiles, id % a.tiles);
+  const Work wk = work_of(a.c.kvh);
+  const uint32_t h = wk.h;
+  if (wk.rest >= a.b.seqs * a.tiles) return;
+  const Tokens tk = tokens_of(a, wk.rest / a.tiles, wk.rest % a.tiles);
   if (tk.n == 0) return;
+  clear_teams(teams);
   score_blocks<D, BF, VEC>(a, tk, h, 0, tk.seen(a, tk.n - 1), lds_keys, a.blocks, codes);
   __syncthreads();
   const size_t out = ((size_t)tk.row * a.c.kvh + h) * a.count;
   if (a.ntok == 1) {
-    choose<kSelWaves>(lds_keys, tk.seen(a, 0), a.count, a.chosen + out, teams[0]);
+    choose<kSelWaves>(lds_keys, tk.seen(a, 0), a.count, a.chosen + out, teams, shared);
   } else {
     const uint32_t wave = threadIdx.x >> 6;
     for (uint32_t t = wave; t < tk.n; t += kSelWaves)
       choose<1>(lds_keys + (size_t)t * a.blocks, tk.seen(a, t), a.count,
-                a.chosen + out + (size_t)t * a.c.kvh * a.count, teams[wave]);
+                a.chosen + out + (size_t)t * a.c.kvh * a.count, teams + wave, shared);
   }
 }
 
@@ -405,11 +472,9 @@ __global__ __launch_bounds__(kSelThreads) void k_select(SelectArgs a) {
 template <int D, bool BF, bool VEC>
 __global__ __launch_bounds__(kSelThreads) void k_score(SelectArgs a) {
   __shared__ __attribute__((aligned(16))) Codes<D> codes;
-  uint32_t id = blockIdx.x;
-  const uint32_t h = id % a.c.kvh;
-  id /= a.c.kvh;
-  const uint32_t chunk = id % a.chunks;
-  id /= a.chunks;
+  const Work wk = work_of(a.c.kvh);
+  const uint32_t h = wk.h, chunk = wk.rest % a.chunks, id = wk.rest / a.chunks;
+  if (id >= a.b.seqs * a.tiles) return;
   const Tokens tk = tokens_of(a, id / a.tiles, id % a.tiles);
   if (tk.n == 0) return;
   const uint32_t from = chunk * a.per, to = min(tk.seen(a, tk.n - 1), from + a.per);
@@ -419,7 +484,8 @@ __global__ __launch_bounds__(kSelThreads) void k_score(SelectArgs a) {
 }
 
 __global__ __launch_bounds__(kSelThreads) void k_top(SelectArgs a) {
-  __shared__ Team team;
+  __shared__ Team teams[kRounds];
+  __shared__ Shared shared;
   const uint32_t h = blockIdx.x % a.c.kvh;
   const uint32_t row = blockIdx.x / a.c.kvh;
   const uint32_t sq = seq_at(a.b, row);
@@ -427,7 +493,9 @@ __global__ __launch_bounds__(kSelThreads) void k_top(SelectArgs a) {
   if (row < s.row || row - s.row >= s.n) return;
   const Tokens tk{sq, row, 1, s.first + (row - s.row), s.len};
   const size_t unit = (size_t)row * a.c.kvh + h;
-  choose<kSelWaves>(a.keys + unit * a.blocks, tk.seen(a, 0), a.count, a.chosen + unit * a.count, team);
+  clear_teams(teams);
+  __syncthreads();
+  choose<kSelWaves>(a.keys + unit * a.blocks, tk.seen(a, 0), a.count, a.chosen + unit * a.count, teams, shared);
 }
 
 }  // namespace
@@ -440,13 +508,14 @@ namespace {
 
 // Keys that a workgroup may keep: 96 KB, so that its counters and others' LDS fit beside it.
 constexpr uint64_t kLdsKeys = 24576;
-// A few long rows: scores by many workgroups, to memory and back.
-constexpr uint64_t kFewUnits = 64, kManyBlocks = 2048;
+// A few long rows: scores by many workgroups, to memory and back. Whole calls, of one
+// workgroup a row and so: 8 rows of 512 blocks 12.5 and 14.0 us, of 1024 16.7 and 14.9, of
+// 2048 24.1 and 16.0; 64 rows of 1024 17.6 and 16.9, 128 rows of 1024 19.4 and 23.4 us.
+constexpr uint64_t kFewUnits = 64, kManyBlocks = 768;
 
 struct SelectPlan {
   bool fused;
   uint32_t gp, ntok, tiles, blocks;
-  uint64_t groups;  // workgroups over sequences and kv heads
 };
 SelectPlan select_plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads) {
   SelectPlan p{};
@@ -457,11 +526,10 @@ SelectPlan select_plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t he
   uint64_t ntok = group > 16 ? 1 : (uint64_t)kRowTiles * (16 / p.gp);
   if (ntok > b->max_tokens) ntok = b->max_tokens;
   const uint64_t units = (uint64_t)b->seqs * c->kv_heads;
-  p.fused = p.blocks <= kLdsKeys && !(b->max_tokens == 1 && units < kFewUnits && p.blocks > kManyBlocks);
+  p.fused = p.blocks <= kLdsKeys && !(b->max_tokens == 1 && units <= kFewUnits && p.blocks > kManyBlocks);
   if (p.fused && ntok * p.blocks > kLdsKeys) ntok = kLdsKeys / p.blocks;
   p.ntok = (uint32_t)ntok;
   p.tiles = (uint32_t)((b->max_tokens + ntok - 1) / ntok);
-  p.groups = units * p.tiles;
   return p;
 }
 
@@ -492,10 +560,11 @@ int dance_kv_select(const DanceKvCache* cache, const DanceKvBatch* batch, const 
   const size_t need = dance_kv_select_work(cache, batch, queries->heads, count);
   if (need && (!work || work_bytes < need || !aligned(work, 16)))
     KV_ERR("dance_kv_select", "work must hold %zu bytes, aligned to 16", need);
-  const uint32_t per = kSelWaves * kTwo * 16u;
+  const uint32_t per = kSelWaves * 16u;
   const uint32_t chunks = p.fused ? 1u : (p.blocks + per - 1) / per;
   const uint64_t units = (uint64_t)batch->tokens * cache->kv_heads;
-  if (p.groups * chunks * kSelThreads > 0xFFFFFFFFull || (!p.fused && units * kSelThreads > 0xFFFFFFFFull))
+  const uint64_t grid = ((uint64_t)batch->seqs * p.tiles * chunks + 7) / 8 * 8 * cache->kv_heads;
+  if (grid * kSelThreads > 0xFFFFFFFFull || (!p.fused && units * kSelThreads > 0xFFFFFFFFull))
     KV_ERR("dance_kv_select", "batch is too large for one launch");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const SelectArgs a{cache_args(cache), batch_args(batch), rows_args(queries), queries->heads / cache->kv_heads, p.gp,
@@ -507,9 +576,9 @@ int dance_kv_select(const DanceKvCache* cache, const DanceKvBatch* batch, const 
       constexpr int D = decltype(d)::value;
       constexpr bool BF = decltype(bf)::value, V = decltype(v)::value;
       if (p.fused)
-        hipLaunchKernelGGL((k_select<D, BF, V>), dim3((uint32_t)p.groups), dim3(kSelThreads), lds, st, a);
+        hipLaunchKernelGGL((k_select<D, BF, V>), dim3((uint32_t)grid), dim3(kSelThreads), lds, st, a);
       else
-        hipLaunchKernelGGL((k_score<D, BF, V>), dim3((uint32_t)(p.groups * chunks)), dim3(kSelThreads), 0, st, a);
+        hipLaunchKernelGGL((k_score<D, BF, V>), dim3((uint32_t)grid), dim3(kSelThreads), 0, st, a);
     };
     vec ? go(std::true_type{}) : go(std::false_type{});
   });
