@@ -699,3 +699,20 @@ def test_library_exports_every_declared_entry():
     assert len(names) == 7
     out = subprocess.run(["nm", "-D", "--defined-only", D.LIB_PATH], capture_output=True, text=True).stdout
     assert {n for n in names if f" T {n}\n" in out} == names
+
+
+@pytest.mark.gpu
+def test_example_of_a_decoding_loop():
+    """The operators together: the selected blocks hold more of the weight than as many of the
+    newest, and all blocks hold all of it."""
+    import os
+    import sys
+    sys.path.insert(0, os.path.join(D.HERE, "..", "examples"))
+    try:
+        import kv_retrieval
+    finally:
+        sys.path.pop(0)
+    some = kv_retrieval.run(seqs=3, prompt=9000, steps=4, count=24, quiet=True)
+    assert all(s["newest"] < s["mass"] <= 1 + 2.0 ** -10 for s in some)
+    every = kv_retrieval.run(seqs=2, prompt=3000, steps=2, count=64, quiet=True)
+    assert all(abs(s["mass"] - 1) < 2.0 ** -10 and s["apart"] < 2.0 ** -7 for s in every)
