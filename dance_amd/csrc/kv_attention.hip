@@ -63,6 +63,8 @@ constexpr uint64_t kChunkUnits = 512;
 constexpr int kChunkWide = 8, kChunkSmall = 4;
 constexpr float kLift = 13.f, kSlack = 2.f;
 constexpr float kLeastScale = 0x1p-100f;  // 2^kLeastExp
+// Least factor of a product: above 0, so that a hidden token's, -infinity, stays that.
+constexpr float kLeastFactor = 0x1p-120f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kSplitUnits = 1024;  // workgroups that fill the chip several times over
 constexpr uint32_t kSplitTiles = 16;    // least tiles of a split: its partial sums are then 2 to 6 % of what it reads
@@ -158,37 +160,32 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
   for (int t = 0; t < DT; ++t) acc[t] = f4_t{0.f, 0.f, 0.f, 0.f};
   float R = -FLT_MAX, l = 0.f;
 
-  // The block with the 16 tokens of group `grp` of a tile, and its first position; a hole: -1.
-  auto locate = [&](uint32_t tt, uint32_t grp, int32_t& first) -> int32_t {
-    const uint32_t vt = tt * kTokTile + grp * 16u;
-    const uint32_t e = vt >> bsh;
-    int32_t lg = -1;
-    if (e < entries) lg = LIST ? list[e] : (int32_t)e;
-    int32_t ph = -1;
-    if (lg >= 0 && lg < seen) ph = table[lg];
-    if ((uint32_t)ph >= a.c.blocks) ph = -1;
-    first = (int32_t)(((uint32_t)lg << bsh) + (vt & (bs - 1u)));
-    return ph;
+  // Loads run ahead in the registers that the products have read: the next
+  // tile's keys set out behind the first product, its values behind the second, the
+  // place of the tile after that one between them, and what a list says of the tile after
+  // that. Nothing that has just been asked for is looked at (loads come back in
+  // order: to look at the last is to wait for all).
+  // Lane group g has the place of its 16 tokens' block: listed (logical), then in the cache (raw).
+  auto listed = [&](uint32_t tt) -> int32_t {
+    const uint32_t e = (tt * kTokTile + g * 16u) >> bsh;
+    return e < entries ? LIST ? list[e] : (int32_t)e : -1;
   };
-  // Loads run a tile ahead in the registers that the products have read: the
-  // next keys set out behind the first product, the next values behind the second, and
-  // the places of the tile after that one between them.
   struct Place {
-    int32_t pk, pv, first;
+    int32_t raw, first;  // first: position of the first of the 16 tokens
   };
-  auto place = [&](uint32_t tt) {
+  auto place = [&](uint32_t tt, int32_t lg) {
     Place p;
-    int32_t other;
-    p.pv = locate(tt, g, p.first);
-    p.pk = locate(tt, n >> 2, other);
+    p.raw = lg >= 0 && lg < seen ? table[lg] : -1;
+    p.first = (int32_t)(((uint32_t)lg << bsh) + ((tt * kTokTile + g * 16u) & (bs - 1u)));
     return p;
   };
+  auto block = [&](const Place& p) -> int32_t { return (uint32_t)p.raw < a.c.blocks ? p.raw : -1; };  // -1: a hole
   uint32_t kw[4][KW];
   u4_t vw[DT];
   float ks, vs;
   auto load_keys = [&](uint32_t tt, const Place& p) {
     const uint32_t slot = (tt * kTokTile + (n >> 2) * 16u) & (bs - 1u);
-    const size_t cell = (size_t)max(p.pk, 0) * a.c.kvh + h;
+    const size_t cell = (size_t)max(__shfl(block(p), (int)((n >> 2) * 16u)), 0) * a.c.kvh + h;
     const int8_t* const kp = a.c.k + ((cell << bsh) + slot + (n & 3u)) * D + g * kPiece;
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
@@ -209,22 +206,27 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
   };
   auto load_values = [&](uint32_t tt, const Place& p) {
     const uint32_t slot = (tt * kTokTile + g * 16u) & (bs - 1u);
-    const size_t cell = (size_t)max(p.pv, 0) * a.c.kvh + h;
+    const size_t cell = (size_t)max(block(p), 0) * a.c.kvh + h;
     const int8_t* const vp = a.c.v + ((cell * D + n) << bsh) + slot;
 #pragma unroll
     for (int t = 0; t < DT; ++t) vw[t] = *reinterpret_cast<const u4_t*>(vp + ((size_t)(16 * t) << bsh));
   };
   auto load_scales = [&](const Place& p) {
-    const size_t cell = (size_t)max(p.pv, 0) * a.c.kvh + h;
-    const float2 x = *reinterpret_cast<const float2*>(a.c.scale + cell * 2);
-    ks = p.pv >= 0 ? x.x : 0.f;
-    vs = p.pv >= 0 ? fmaxf(x.y, kLeastScale) : 1.f;
+    const float2 x = *reinterpret_cast<const float2*>(a.c.scale + ((size_t)max(block(p), 0) * a.c.kvh + h) * 2);
+    ks = x.x;
+    vs = x.y;
   };
 
   uint32_t tt = split * a.per + wave;
   const bool any = tt < t_end;
   Place here, next;
-  if (any) here = place(tt);
+  int32_t then = -1;
+  if (any) {
+    const int32_t l0 = listed(tt), l1 = listed(tt + W);
+    then = listed(tt + 2 * W);
+    here = place(tt, l0);
+    next = place(tt + W, l1);
+  }
   u4_t raw[KS];
   {
     const uint16_t* src = a.q.data + (int64_t)(s.row + tok) * a.q.token_stride + (int64_t)head * a.q.head_stride + g * kPiece;
@@ -243,11 +245,12 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
     load_scales(here);
     load_keys(tt, here);
     load_values(tt, here);
-    next = place(tt + W);
   }
-  // Queries, as f16 with a power of two taken out so that bf16's range fits.
+  // Queries, as f16 with a power of two taken out so that bf16's range fits. A negative
+  // scale turns them over, so that the largest product has the largest logit.
   h8_t qf[KS];
-  float qscale = a.scale2;
+  float qscale = fabsf(a.scale2);
+  const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;
   if constexpr (BF) {
     float mag = 0.f;
 #pragma unroll
@@ -263,16 +266,26 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
     for (int c = 0; c < KS; ++c)
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        qf[c][i] = (_Float16)(load_val<true>((uint16_t)(raw[c][i >> 1] >> (16 * (i & 1)))) * inv);
+        qf[c][i] = (_Float16)(load_val<true>((uint16_t)((raw[c][i >> 1] ^ flip) >> (16 * (i & 1)))) * inv);
   } else {
 #pragma unroll
-    for (int c = 0; c < KS; ++c) qf[c] = __builtin_bit_cast(h8_t, raw[c]);
+    for (int c = 0; c < KS; ++c) qf[c] = __builtin_bit_cast(h8_t, raw[c] ^ u4_t{flip, flip, flip, flip});
   }
+  // What the key operand has too much, 128 for each code (small8), in its products.
+  float q_off = 0.f;
+#pragma unroll
+  for (int c = 0; c < KS; ++c)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q_off += (float)qf[c][i];
+  q_off = rows_sum(q_off) * (-128.f * 0x1p-24f);
 
   for (; tt < t_end; tt += W) {
     // tokens of this lane that its row sees: the first `lim` + 1 of its 16
-    const int32_t lim = here.pv >= 0 && here.first <= pos ? pos - here.first : -1;
-    const float kq = ks * qscale, lv = __builtin_amdgcn_logf(vs), iv = 1.f / vs;
+    const bool hole = block(here) < 0;
+    const int32_t lim = !hole && here.first <= pos ? pos - here.first : -1;
+    const float y = hole ? 1.f : fmaxf(vs, kLeastScale), iv = 1.f / y;
+    const float kq = fmaxf(hole ? 0.f : ks * 0x1p24f * qscale, kLeastFactor);
+    const float lv = __builtin_fmaf(kq, q_off, __builtin_amdgcn_logf(y));
     const bool more = tt + W < t_end;
     f4_t sc[4];
 #pragma unroll
@@ -280,20 +293,25 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
       sc[st] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < KS; ++c)
-        sc[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(kw[st][2 * c], kw[st][2 * c + 1]), qf[c], sc[st], 0, 0, 0);
+        sc[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(small8(kw[st][2 * c], kw[st][2 * c + 1]), qf[c], sc[st], 0, 0, 0);
     }
     if (more) {
       load_scales(next);
       load_keys(tt + W, next);
     }
-    float big = -FLT_MAX;
+    if (__any(lim < 15)) {
+#pragma unroll
+      for (int st = 0; st < 4; ++st)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (4 * st + i > lim) sc[st][i] = -__builtin_inff();
+    }
+    float most = -__builtin_inff();
 #pragma unroll
     for (int st = 0; st < 4; ++st)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sc[st][i] = 4 * st + i <= lim ? __builtin_fmaf(sc[st][i], kq, lv) : -__builtin_inff();
-        big = fmaxf(big, sc[st][i]);
-      }
+      for (int i = 0; i < 4; ++i) most = fmaxf(most, sc[st][i]);
+    const float big = __builtin_fmaf(most, kq, lv);
     if (__any(big > R + (kLift + kSlack))) {
       // each row by its own logits alone: a row's result does not depend on its neighbours
       const float row_big = rows_max(big);
@@ -308,11 +326,12 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
     }
     h8_t pf[2];
     float add = 0.f;
+    const float off = lv - R;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float p = __builtin_amdgcn_exp2f(sc[2 * u + (i >> 2)][i & 3] - R);
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * u + (i >> 2)][i & 3], kq, off));
         add += p;
         pf[u][i] = (_Float16)p;
       }
@@ -324,7 +343,8 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
     }
     if (more) {
       here = next;
-      next = place(tt + 2 * W);
+      next = place(tt + 2 * W, then);
+      then = listed(tt + 3 * W);
       load_values(tt + W, here);
     }
   }

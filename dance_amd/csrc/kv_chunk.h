@@ -12,9 +12,6 @@
 // operand wants: within 16 tokens 0-3, 8-11, 4-7, 12-15, a swap of words.
 #pragma once
 
-// Least factor of a product: above 0, so that a hidden token's, -infinity, stays that.
-constexpr float kLeastFactor = 0x1p-120f;
-
 constexpr int chunk_occ(int d) { return d <= 128 ? 2 : 1; }  // waves per SIMD, by registers
 
 typedef float f16_t __attribute__((ext_vector_type(16)));
