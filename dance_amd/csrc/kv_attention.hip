@@ -91,8 +91,11 @@ __device__ __forceinline__ float lse_of(float R, float l) {
   return l < __builtin_inff() ? ((R + e) + log2f(m)) * kLn2 : l;  // l is normal, infinite or NaN
 }
 
+constexpr int step_occ(int d) { return d <= 192 ? 2 : 1; }  // waves per SIMD, by registers
+
 template <int D, bool BF, bool LIST, bool VEC, uint32_t W>
-__global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(step_occ(D), step_occ(D)))) void k_step(
+    StepArgs a) {
   constexpr int KS = D / 32;  // inner steps of the first product
   constexpr int DT = D / 16;  // row tiles of the second
   constexpr int KW = D / 16;  // words of a key row that a lane holds
@@ -338,6 +341,7 @@ __global__ __launch_bounds__(64 * W) void k_step(StepArgs a) {
     l += add * iv;
 #pragma unroll
     for (int t = 0; t < DT; ++t) {
+      asm volatile("" : "+v"(vw[t]));  // values are waited for here, not where their conversion could begin
       acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vw[t].x, vw[t].y), pf[0], acc[t], 0, 0, 0);
       acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vw[t].z, vw[t].w), pf[1], acc[t], 0, 0, 0);
     }
