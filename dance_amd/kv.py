@@ -26,6 +26,7 @@ ready on this one. There is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -52,9 +53,15 @@ class DanceKvRows(C.Structure):
                 ("dtype", C.c_int)]
 
 
-_bound = None
+# The same structs as bytes, which a call takes as it takes a pointer: a small
+# attention is 8 us of host time, and the three ctypes objects would be another 1.5.
+_CACHE, _BATCH, _ROWS = struct.Struct("@PPPPIIII"), struct.Struct("@PPPIIIIQ"), struct.Struct("@PqqIi")
+assert [_CACHE.size, _BATCH.size, _ROWS.size] == [C.sizeof(t) for t in (DanceKvCache, DanceKvBatch, DanceKvRows)]
+
 # torch's handle of the current stream, without the Stream object around it where torch has that
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_bound = None
+_fast = {}
 
 
 def _stream(index):
@@ -77,6 +84,8 @@ def _bind():
                 ("sparse_attention_work", [cache, batch, u32, u32], sz)):
             fn = getattr(L, "dance_kv_" + name)
             fn.argtypes, fn.restype = args, res
+            as_bytes = [C.c_char_p if t in (cache, batch, rows) else t for t in args]
+            _fast[name] = C.CFUNCTYPE(res, *as_bytes)(("dance_kv_" + name, L))
         _bound = L
     return _bound
 
@@ -111,9 +120,9 @@ class KVCache:
         self.k, self.v, self.scale, self.bound = k, v, scale, bound
         self.blocks, self.kv_heads, self.block_tokens, self.dim = blocks, heads, block_tokens, dim
         self.device = k.device
-        self._c = DanceKvCache(k.data_ptr(), v.data_ptr(), scale.data_ptr(), bound.data_ptr(), blocks, heads, dim,
-                               block_tokens)
-        self._ref = C.byref(self._c)
+        self._bytes = _CACHE.pack(k.data_ptr(), v.data_ptr(), scale.data_ptr(), bound.data_ptr(), blocks, heads, dim,
+                                  block_tokens)
+        _bind()
 
     @classmethod
     def empty(cls, blocks, kv_heads, dim, block_tokens=64, device="cuda"):
@@ -128,60 +137,66 @@ class KVCache:
 def _ints(name, t, shape, device):
     if t.dtype != torch.int32:
         raise TypeError(f"{name} must be int32")
-    if t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous and on the cache's device")
     if t.shape != shape:
         raise ValueError(f"{name} must have the shape {tuple(shape)}")
+    if t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous and on the cache's device")
 
 
 def _rows(cache, name, t, heads=None):
-    if t.ndim != 3 or t.shape[2] != cache.dim:
+    """Checks rows of keys, values or queries; (their struct's bytes, tokens, heads)."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != cache.dim:
         raise ValueError(f"{name} must be [tokens, heads, {cache.dim}]")
-    if t.dtype not in DTYPES:
+    dtype = DTYPES.get(t.dtype)
+    if dtype is None:
         raise TypeError(f"{name} must be float16 or bfloat16")
     if t.device != cache.device:
         raise ValueError(f"{name} must be on the cache's device")
-    st = t.stride()
-    if st[2] != 1:
+    token_stride, head_stride, one = t.stride()
+    if one != 1:
         raise ValueError(f"the dimensions of {name} must be adjacent")
-    n = t.shape[1]
+    tokens, n, _ = shape
     if n != heads if heads else n == 0 or n % cache.kv_heads:
         raise ValueError(f"{name} must have {heads} heads" if heads else
                          f"{name} must have a multiple of {cache.kv_heads} heads")
-    return DanceKvRows(t.data_ptr(), st[0], st[1], n, DTYPES[t.dtype])
+    return _ROWS.pack(t.data_ptr(), token_stride, head_stride, n, dtype), tokens, n
 
 
-def _batch(cache, rows, table, lengths, offsets, max_tokens, max_length):
-    if table.ndim != 2:
+def _batch(cache, tokens, table, lengths, offsets, max_tokens, max_length):
+    """Checks a batch; its struct's bytes."""
+    shape = table.shape
+    if len(shape) != 2:
         raise ValueError("table must be [sequences, blocks]")
-    tokens, (seqs, width) = rows.shape[0], table.shape
-    _ints("table", table, (seqs, width), cache.device)
+    seqs, width = shape
+    _ints("table", table, shape, cache.device)
     _ints("lengths", lengths, (seqs,), cache.device)
     if offsets is None:
         if tokens != seqs:
             raise ValueError("without offsets there is one row for each sequence")
-        max_tokens = 1
+        max_tokens, at = 1, 0
     else:
         _ints("offsets", offsets, (seqs + 1,), cache.device)
         if max_tokens is None:
             max_tokens = tokens
         elif max_tokens < 1:
             raise ValueError("max_tokens must be positive")
+        at = offsets.data_ptr()
     if max_length is not None and max_length < 1:
         raise ValueError("max_length must be positive")
-    return DanceKvBatch(table.data_ptr(), lengths.data_ptr(), offsets.data_ptr() if offsets is not None else None, seqs,
-                        tokens, width, min(max_tokens, tokens), max_length or 0)
+    return _BATCH.pack(table.data_ptr(), lengths.data_ptr(), at, seqs, tokens, width, min(max_tokens, tokens),
+                       max_length or 0)
 
 
 def _call(name, cache, *args):
-    fn, index = getattr(_bound, name), cache.device.index
+    index = cache.device.index
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
-            rc = fn(cache._ref, *args, _stream(index))
+            rc = _fast[name](cache._bytes, *args, _stream(index))
     else:
-        rc = fn(cache._ref, *args, _stream(index))
+        rc = _fast[name](cache._bytes, *args, _stream(index))
     if rc != 0:
-        raise RuntimeError(f"{name} failed with return code {rc}")
+        raise RuntimeError(f"dance_kv_{name} failed with return code {rc}")
 
 
 def _work(cache, size):
@@ -192,23 +207,23 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _out(name, t, shape, dtype, device):
+def _out(t, q):
     if t is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on the cache's device")
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device or not t.is_contiguous():
+        raise ValueError(f"out must be a contiguous {q.dtype} tensor of q's shape on the cache's device")
     return t
 
 
 def append(cache, k, v, table, lengths, offsets=None, max_tokens=None):
     """Writes the rows' keys and values into the cache's blocks; scales and bounds follow."""
-    kr, vr = _rows(cache, "k", k, cache.kv_heads), _rows(cache, "v", v, cache.kv_heads)
-    if k.shape != v.shape or k.dtype != v.dtype:
+    kr, tokens, _ = _rows(cache, "k", k, cache.kv_heads)
+    vr, others, _ = _rows(cache, "v", v, cache.kv_heads)
+    if tokens != others or k.dtype != v.dtype:
         raise ValueError("k and v must have one shape and type")
-    b = _batch(cache, k, table, lengths, offsets, max_tokens, None)
-    _bind()
-    if k.shape[0]:
-        _call("dance_kv_append", cache, C.byref(b), C.byref(kr), C.byref(vr))
+    b = _batch(cache, tokens, table, lengths, offsets, max_tokens, None)
+    if tokens:
+        _call("append", cache, b, kr, vr)
 
 
 def attention(cache, q, table, lengths, offsets=None, *, scale=None, max_tokens=None, max_length=None, out=None,
@@ -217,15 +232,15 @@ def attention(cache, q, table, lengths, offsets=None, *, scale=None, max_tokens=
     dim] of q's type. With return_lse also the logarithm of each row's sum
     [tokens, heads] in float32. Rows that see nothing give zeros and -inf.
     scale defaults to dim ** -0.5."""
-    r = _rows(cache, "q", q)
-    b = _batch(cache, q, table, lengths, offsets, max_tokens, max_length)
-    out = _out("out", out, q.shape, q.dtype, cache.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=cache.device) if return_lse else None
-    if q.shape[0]:
-        size = _bind().dance_kv_attention_work(cache._ref, C.byref(b), r.heads)
+    r, tokens, heads = _rows(cache, "q", q)
+    b = _batch(cache, tokens, table, lengths, offsets, max_tokens, max_length)
+    out = _out(out, q)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=cache.device) if return_lse else None
+    if tokens:
+        size = _fast["attention_work"](cache._bytes, b, heads)
         work = _work(cache, size)
-        _call("dance_kv_attention", cache, C.byref(b), C.byref(r), cache.dim ** -0.5 if scale is None else scale,
-              out.data_ptr(), _ptr(lse), _ptr(work), size)
+        _call("attention", cache, b, r, cache.dim ** -0.5 if scale is None else scale, out.data_ptr(), _ptr(lse),
+              _ptr(work), size)
     return (out, lse) if return_lse else out
 
 
@@ -236,15 +251,15 @@ def select(cache, q, table, lengths, count, offsets=None, *, sink=0, recent=0, m
     in ascending order, -1 behind them. Equal bounds go to the lower block. The
     first `sink` and the last `recent` blocks that a row sees are always among
     them."""
-    r = _rows(cache, "q", q)
-    b = _batch(cache, q, table, lengths, offsets, max_tokens, max_length)
+    r, tokens, heads = _rows(cache, "q", q)
+    b = _batch(cache, tokens, table, lengths, offsets, max_tokens, max_length)
     if count < 1 or sink < 0 or recent < 0 or sink + recent > count:
         raise ValueError("count must be positive and hold sink and recent")
-    chosen = torch.empty((q.shape[0], cache.kv_heads, count), dtype=torch.int32, device=cache.device)
-    if q.shape[0]:
-        size = _bind().dance_kv_select_work(cache._ref, C.byref(b), r.heads, count)
+    chosen = torch.empty((tokens, cache.kv_heads, count), dtype=torch.int32, device=cache.device)
+    if tokens:
+        size = _fast["select_work"](cache._bytes, b, heads, count)
         work = _work(cache, size)
-        _call("dance_kv_select", cache, C.byref(b), C.byref(r), count, sink, recent, chosen.data_ptr(), _ptr(work), size)
+        _call("select", cache, b, r, count, sink, recent, chosen.data_ptr(), _ptr(work), size)
     return chosen
 
 
@@ -253,17 +268,17 @@ def sparse_attention(cache, q, chosen, table, lengths, offsets=None, *, scale=No
     """attention over the blocks that `chosen` [tokens, kv_heads, count] int32 lists
     for each row and kv head: logical blocks in any order, each at most once;
     negative ones and those the row does not see are left out."""
-    r = _rows(cache, "q", q)
-    b = _batch(cache, q, table, lengths, offsets, max_tokens, None)
+    r, tokens, heads = _rows(cache, "q", q)
+    b = _batch(cache, tokens, table, lengths, offsets, max_tokens, None)
     if chosen.ndim != 3 or chosen.shape[2] < 1:
         raise ValueError("chosen must be [tokens, kv_heads, count]")
     count = chosen.shape[2]
-    _ints("chosen", chosen, (q.shape[0], cache.kv_heads, count), cache.device)
-    out = _out("out", out, q.shape, q.dtype, cache.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=cache.device) if return_lse else None
-    if q.shape[0]:
-        size = _bind().dance_kv_sparse_attention_work(cache._ref, C.byref(b), r.heads, count)
+    _ints("chosen", chosen, (tokens, cache.kv_heads, count), cache.device)
+    out = _out(out, q)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=cache.device) if return_lse else None
+    if tokens:
+        size = _fast["sparse_attention_work"](cache._bytes, b, heads, count)
         work = _work(cache, size)
-        _call("dance_kv_sparse_attention", cache, C.byref(b), C.byref(r), chosen.data_ptr(), count,
-              cache.dim ** -0.5 if scale is None else scale, out.data_ptr(), _ptr(lse), _ptr(work), size)
+        _call("sparse_attention", cache, b, r, chosen.data_ptr(), count, cache.dim ** -0.5 if scale is None else scale,
+              out.data_ptr(), _ptr(lse), _ptr(work), size)
     return (out, lse) if return_lse else out
