@@ -7,6 +7,7 @@
 
 #include <cstdint>
 #include <cstdio>
+#include <type_traits>
 
 #include "../../include/dance_kv.h"
 
@@ -158,6 +159,17 @@ __device__ __forceinline__ float rows_max(float x) {
   x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
   const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+// Over the 16 lanes that differ in bits 0 to 3.
+__device__ __forceinline__ float cols_max(float x) {
+  auto with = [&](auto ctrl) {  // quad lanes 1 0 3 2, then 2 3 0 1, half rows mirrored, rows mirrored
+    x = fmaxf(x, __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), decltype(ctrl)::value, 0xF, 0xF, true)));
+  };
+  with(std::integral_constant<int, 0xB1>{});
+  with(std::integral_constant<int, 0x4E>{});
+  with(std::integral_constant<int, 0x141>{});
+  with(std::integral_constant<int, 0x140>{});
+  return x;
 }
 // Over the two lanes that differ in bit 4.
 __device__ __forceinline__ float pair_max(float x) {

@@ -104,8 +104,7 @@ __device__ __forceinline__ void code_rows(const SelectArgs& a, const Tokens& tk,
     float mag = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) mag = fmaxf(mag, finite_abs(x[i]));
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) mag = fmaxf(mag, __shfl_xor(mag, d));
+    mag = cols_max(mag);
     const int e = scale_exp(mag);
     const float inv = exp2_int(-e);
     int8_t* const out = qc.c + r * Codes<D>::kStride + l * V;
