@@ -76,7 +76,7 @@ struct StepArgs {
   const int32_t* __restrict__ lists;  // LIST: tokens x kv_heads x count
   uint32_t count;
   float scale2;  // scale * log2(e)
-  uint32_t group, tiles, outer, splits, per;  // per: tiles of 64 tokens in a split
+  uint32_t group, tiles, slots, splits, per;  // row tiles of a sequence (0: see tile_at), of all; 64 tokens of a split
   uint16_t* __restrict__ out;
   float* __restrict__ lse;
   float* __restrict__ part;  // splits > 1: [row][split][D] sums, then [row][split][2] (R, l)
@@ -112,12 +112,18 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(step_occ
   // fastest, 8 of them: 215 us for a ragged batch that takes 120 like this).
   const uint32_t h = id % a.c.kvh;
   id /= a.c.kvh;
-  const uint32_t tile = id % a.tiles;
-  id /= a.tiles;
-  const uint32_t split = id / a.outer;
-  id %= a.outer;
-  // id: the token row (LIST) or the sequence
-  const uint32_t sq = LIST ? seq_at(a.b, id) : id;
+  const uint32_t split = id / a.slots;
+  id %= a.slots;
+  TileAt at;
+  if constexpr (LIST) {
+    at.tile = id % a.tiles;
+    id /= a.tiles;  // the token row
+    at.sq = seq_at(a.b, id);
+  } else {
+    at = tile_at(a.b, id, a.group, kRowTile, a.tiles);
+    if (at.sq >= a.b.seqs) return;
+  }
+  const uint32_t sq = at.sq, tile = at.tile;
   const Seq s = seq_of(a.b, sq, bsh);
   // rows of the tile: index r counts (token, head of the group), tokens slowest
   uint32_t r_first, r_end;
@@ -137,8 +143,17 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(step_occ
   const int64_t p_row = min(s.first + tok, s.len - 1), p_top = min(s.first + (r_first + rows - 1) / a.group, s.len - 1);
   const int32_t pos = n < rows && p_row >= 0 ? (int32_t)p_row : -1, top = p_top >= 0 ? (int32_t)p_top : -1;
   const int32_t seen = (int32_t)((uint32_t)(top + 1 + (int32_t)bs - 1) >> bsh);  // blocks
-  const uint32_t entries = LIST ? a.count : (uint32_t)seen;
   const int32_t* const list = LIST ? a.lists + ((size_t)id * a.c.kvh + h) * a.count : nullptr;
+  uint32_t entries = (uint32_t)seen;
+  if constexpr (LIST) {  // up to the last one that the row sees: a selection of few blocks ends in -1
+    entries = 0;
+    for (uint32_t e0 = 0; e0 < a.count; e0 += 64) {
+      const int32_t lg = e0 + lane < a.count ? list[e0 + lane] : -1;
+      const uint64_t mask = __ballot(lg >= 0 && lg < seen);
+      if (mask) entries = e0 + 64u - (uint32_t)__clzll((long long)mask);
+    }
+    entries = (uint32_t)__builtin_amdgcn_readfirstlane((int)entries);
+  }
   const int32_t* const table = a.b.table + (size_t)sq * a.b.width;
 
   // this split's tiles of 64 listed tokens
@@ -467,8 +482,8 @@ __global__ __launch_bounds__(64 * (W == 1 ? kJoinRows : W)) void k_join(const fl
 }
 
 struct Plan {
-  uint64_t units;  // sequences or token rows, x row tiles x kv heads
-  uint32_t tiles, splits, per;
+  uint64_t units;  // row tiles of all sequences or token rows, x kv heads
+  uint32_t tiles, slots, splits, per;
   bool wide, chunk;
   int waves;  // of a workgroup of k_chunk
   size_t work;
@@ -484,7 +499,9 @@ Plan plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, bool lis
   p.waves = c->dim <= 128 && (group * b->tokens + big - 1) / big * c->kv_heads >= kChunkUnits ? kChunkWide : kChunkSmall;
   const uint32_t row_tile = p.chunk ? 32u * p.waves : kRowTile;
   p.tiles = (uint32_t)((rows + row_tile - 1) / row_tile);
-  p.units = (uint64_t)(list ? b->tokens : b->seqs) * p.tiles * c->kv_heads;
+  const uint64_t slots = list ? (uint64_t)b->tokens * p.tiles : tile_slots(b, group, row_tile, p.tiles);
+  p.slots = (uint32_t)slots;
+  p.units = slots * c->kv_heads;
   // A split takes a fixed number of tiles, so that sequences of other lengths take
   // other numbers of workgroups.
   const uint64_t all = ((uint64_t)(list ? count : most_blocks(c, b)) * c->block_tokens + kTokTile - 1) / kTokTile;
@@ -494,9 +511,8 @@ Plan plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, bool lis
     p.splits = 1;
     return p;
   }
-  const uint64_t there = p.chunk ? (group * b->tokens + row_tile - 1) / row_tile * c->kv_heads : p.units;
   const uint64_t want = p.chunk ? kChunkUnits : kSplitUnits, round = p.chunk ? 1 : kStepWaves;
-  uint64_t per = there * 2 >= want && p.chunk ? all : (there * all + want - 1) / want;
+  uint64_t per = p.chunk && p.units * 2 >= want ? all : (p.units * all + want - 1) / want;
   const uint64_t least = p.chunk ? kChunkSplitTiles : kSplitTiles;
   per = per < least ? least : (per + round - 1) / round * round;
   p.per = (uint32_t)(per < all ? per : all);
@@ -524,16 +540,14 @@ int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, c
     std::fprintf(stderr, "[%s] work must hold %zu bytes, aligned to 16\n", who, p.work);
     return -1;
   }
-  // k_chunk deals sequences and heads out eight at a time
-  const uint64_t pairs = (uint64_t)batch->seqs * cache->kv_heads;
-  const uint64_t grid = p.chunk && pairs > 8 ? (pairs + 7) / 8 * 8 * p.tiles * p.splits : p.units * p.splits;
+  const uint64_t grid = p.units * p.splits;
   if (grid * 64 * 8 > 0xFFFFFFFFull || (uint64_t)batch->tokens * q->heads * 64 * kJoinWaves > 0xFFFFFFFFull) {
     std::fprintf(stderr, "[%s] batch is too large for one launch\n", who);
     return -1;
   }
   const hipStream_t st = static_cast<hipStream_t>(stream);
   StepArgs a{cache_args(cache), batch_args(batch), rows_args(q), lists, count, scale * kLog2e,
-             q->heads / cache->kv_heads, p.tiles, list ? batch->tokens : batch->seqs, p.splits, p.per, static_cast<uint16_t*>(out), lse,
+             q->heads / cache->kv_heads, p.tiles, p.slots, p.splits, p.per, static_cast<uint16_t*>(out), lse,
              static_cast<float*>(work)};
   const bool vec = rows_vector(q);
   with_kind(cache->dim, q->dtype, [&](auto d, auto bf) {

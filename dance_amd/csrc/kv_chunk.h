@@ -42,21 +42,19 @@ __global__ __launch_bounds__(64 * W)
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t n = lane & 31u, hl = lane >> 5;
   const uint32_t bsh = a.c.bsh, bs = 1u << bsh;
-  // Sequences and heads go round the XCDs, so that the workgroups that read the
-  // same tokens share an L2; last rows, which see the most, first.
+  // Heads go round the XCDs, so that the workgroups that read the same tokens
+  // share an L2 (with eight heads); a sequence's last rows, which see the most, first.
   uint32_t id = blockIdx.x;
-  const uint32_t units = a.outer * a.c.kvh, fast = min(units, 8u);
-  const uint32_t low = id % fast;
-  id /= fast;
-  const uint32_t tile = a.tiles - 1u - id % a.tiles;
-  id /= a.tiles;
-  const uint32_t split = id % a.splits;
-  const uint32_t unit = id / a.splits * fast + low;
-  if (unit >= units) return;
-  const uint32_t h = unit % a.c.kvh, sq = unit / a.c.kvh;
+  const uint32_t h = id % a.c.kvh;
+  id /= a.c.kvh;
+  const uint32_t split = id / a.slots;
+  const TileAt at = tile_at(a.b, id % a.slots, a.group, kRows, a.tiles);
+  if (at.sq >= a.b.seqs) return;
+  const uint32_t sq = at.sq;
   const Seq s = seq_of(a.b, sq, bsh);
-  const uint32_t r_first = tile * kRows, r_end = s.n * a.group;
-  if (r_first >= r_end) return;
+  const uint32_t r_end = s.n * a.group, tiles = (r_end + kRows - 1u) / kRows;
+  if (at.tile >= tiles) return;
+  const uint32_t r_first = (tiles - 1u - at.tile) * kRows;
   const uint32_t rows = min(kRows, r_end - r_first);
   auto pos_of = [&](uint32_t r) {
     const int64_t p = min(s.first + r / a.group, s.len - 1);

@@ -92,6 +92,35 @@ __device__ __forceinline__ uint32_t less(uint32_t a, uint32_t b) {
   return d > 0 ? (uint32_t)d : 0u;
 }
 
+// Tiles of `per` of a sequence's rows x `group`, of all sequences in one index: a
+// sequence of n has the indexes from slot(b) = offset * group / per + b up to slot(b +
+// 1), at least as many as its tiles. So a grid goes by the rows that there are and not by the
+// longest sequence's; where that is no fewer, each sequence has `tiles` (not 0). sq = seqs: no such tile.
+struct TileAt {
+  uint32_t sq, tile;
+};
+__device__ __forceinline__ TileAt tile_at(const Batch& b, uint32_t id, uint32_t group, uint32_t per, uint32_t tiles) {
+  if (tiles) return TileAt{id / tiles, id % tiles};
+  auto slot = [&](uint32_t i) { return (uint32_t)max(b.offsets[i], 0) * group / per + i; };
+  uint32_t before = 0;  // sequences whose indexes begin at or before this one
+  for (uint32_t i0 = 0; i0 < b.seqs; i0 += 64) {
+    const uint32_t i = i0 + (threadIdx.x & 63u);
+    const uint64_t mask = __ballot(i < b.seqs && slot(min(i, b.seqs - 1u)) <= id);
+    before += (uint32_t)__popcll(mask);
+    if (mask != ~0ull) break;
+  }
+  const uint32_t sq = (uint32_t)__builtin_amdgcn_readfirstlane((int)(before - 1u));
+  if (sq >= b.seqs) return TileAt{b.seqs, 0};
+  return TileAt{sq, id - slot(sq)};
+}
+// The indexes of a grid, and 0 for `tiles` where they go by the rows.
+inline uint64_t tile_slots(const DanceKvBatch* b, uint64_t group, uint64_t per, uint32_t& tiles) {
+  const uint64_t by_rows = b->tokens * group / per + b->seqs, by_longest = (uint64_t)b->seqs * tiles;
+  if (!b->offsets || by_longest <= by_rows) return by_longest;
+  tiles = 0;
+  return by_rows;
+}
+
 template <bool BF>
 __device__ __forceinline__ float load_val(uint16_t u) {
   if constexpr (BF)

@@ -41,7 +41,7 @@ struct SelectArgs {
   Batch b;
   Rows q;
   uint32_t group, gp;    // heads of a kv head; padded to a power of two where they share a row tile
-  uint32_t ntok, tiles;  // token rows of a workgroup, workgroups of a sequence
+  uint32_t ntok, tiles, slots;  // token rows of a workgroup, workgroups of a sequence (0: see tile_at), of all
   uint32_t count, sink, recent;
   uint32_t blocks;       // keys of a token row
   uint32_t chunks, per;  // k_score: workgroups that share the blocks, blocks of each
@@ -450,8 +450,10 @@ __global__ __launch_bounds__(kSelThreads) void k_select(SelectArgs a) {
   __shared__ __attribute__((aligned(16))) Codes<D> codes;
   const Work wk = work_of(a.c.kvh);
   const uint32_t h = wk.h;
-  if (wk.rest >= a.b.seqs * a.tiles) return;
-  const Tokens tk = tokens_of(a, wk.rest / a.tiles, wk.rest % a.tiles);
+  if (wk.rest >= a.slots) return;
+  const TileAt at = tile_at(a.b, wk.rest, 1, a.ntok, a.tiles);
+  if (at.sq >= a.b.seqs) return;
+  const Tokens tk = tokens_of(a, at.sq, at.tile);
   if (tk.n == 0) return;
   clear_teams(teams);
   score_blocks<D, BF, VEC>(a, tk, h, 0, tk.seen(a, tk.n - 1), lds_keys, a.blocks, codes);
@@ -473,8 +475,10 @@ __global__ __launch_bounds__(kSelThreads) void k_score(SelectArgs a) {
   __shared__ __attribute__((aligned(16))) Codes<D> codes;
   const Work wk = work_of(a.c.kvh);
   const uint32_t h = wk.h, chunk = wk.rest % a.chunks, id = wk.rest / a.chunks;
-  if (id >= a.b.seqs * a.tiles) return;
-  const Tokens tk = tokens_of(a, id / a.tiles, id % a.tiles);
+  if (id >= a.slots) return;
+  const TileAt at = tile_at(a.b, id, 1, a.ntok, a.tiles);
+  if (at.sq >= a.b.seqs) return;
+  const Tokens tk = tokens_of(a, at.sq, at.tile);
   if (tk.n == 0) return;
   const uint32_t from = chunk * a.per, to = min(tk.seen(a, tk.n - 1), from + a.per);
   if (from < to)
@@ -514,7 +518,7 @@ constexpr uint64_t kFewUnits = 64, kManyBlocks = 768;
 
 struct SelectPlan {
   bool fused;
-  uint32_t gp, ntok, tiles, blocks;
+  uint32_t gp, ntok, tiles, slots, blocks;
 };
 SelectPlan select_plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads) {
   SelectPlan p{};
@@ -529,6 +533,7 @@ SelectPlan select_plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t he
   if (p.fused && ntok * p.blocks > kLdsKeys) ntok = kLdsKeys / p.blocks;
   p.ntok = (uint32_t)ntok;
   p.tiles = (uint32_t)((b->max_tokens + ntok - 1) / ntok);
+  p.slots = (uint32_t)tile_slots(b, 1, ntok, p.tiles);
   return p;
 }
 
@@ -562,12 +567,12 @@ int dance_kv_select(const DanceKvCache* cache, const DanceKvBatch* batch, const 
   const uint32_t per = kSelWaves * 16u;
   const uint32_t chunks = p.fused ? 1u : (p.blocks + per - 1) / per;
   const uint64_t units = (uint64_t)batch->tokens * cache->kv_heads;
-  const uint64_t grid = ((uint64_t)batch->seqs * p.tiles * chunks + 7) / 8 * 8 * cache->kv_heads;
+  const uint64_t grid = ((uint64_t)p.slots * chunks + 7) / 8 * 8 * cache->kv_heads;
   if (grid * kSelThreads > 0xFFFFFFFFull || (!p.fused && units * kSelThreads > 0xFFFFFFFFull))
     KV_ERR("dance_kv_select", "batch is too large for one launch");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const SelectArgs a{cache_args(cache), batch_args(batch), rows_args(queries), queries->heads / cache->kv_heads, p.gp,
-                     p.ntok, p.tiles, count, sink, recent, p.blocks, chunks, per, static_cast<uint32_t*>(work), chosen};
+                     p.ntok, p.tiles, p.slots, count, sink, recent, p.blocks, chunks, per, static_cast<uint32_t*>(work), chosen};
   const bool vec = rows_vector(queries);
   const size_t lds = (size_t)p.ntok * p.blocks * 4;
   with_kind(cache->dim, queries->dtype, [&](auto d, auto bf) {
