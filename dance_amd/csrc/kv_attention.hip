@@ -1,6 +1,6 @@
 // dance_kv_attention and dance_kv_sparse_attention (include/dance_kv.h).
 //
-// For a tile of 64 tokens and 16 query rows a wave forms S' = K Q' (tokens x
+// For a tile of 64 tokens (32 at 256 dimensions) and 16 query rows a wave forms S' = K Q' (tokens x
 // rows) and then O' += V' P' (dims x rows) with 16x16x32 f16 MFMAs. Codes are
 // whole numbers below 2^11, so they are exact in f16, and the scales stay out
 // of the products: a key's scale multiplies its logit, a value's the weight.
@@ -40,20 +40,21 @@ constexpr uint32_t kStepWaves = 4;
 constexpr uint32_t kJoinWaves = 8, kJoinRows = 4;  // waves on a row, or rows of a workgroup
 constexpr uint32_t kJoinFew = 16;                 // splits that one wave joins
 constexpr uint32_t kRowTile = 16;
-constexpr uint32_t kTokTile = 64;
-// Waves of a workgroup that takes all of a row tile's tokens: what the registers allow.
-constexpr uint32_t wide_waves(int d) { return d <= 192 ? 8 : 4; }
-// It needs no join (and its launch), but a CU reads 75 GB/s at most: up to one
-// workgroup per CU and kWideBytes of codes for each, more where many keep the chip
-// busy anyway. Measured with it and with splits, of 128 dimensions (whole calls): 8 units of 1024
-// tokens 11.6 and 13.5 us, of 2048 16.7 and 14.1 us; kernels alone: 216 units of 3500 x 64
-// (448 KB) 16.0 and 13.8 + 3.9 us, 128 of 4096 x 128 (1 MB) 42.5 and 31.0 + 4.1 us.
+// Waves of a workgroup that takes all of a row tile's tokens. It needs no join (and
+// its launch), but a CU reads 75 GB/s at most: up to one workgroup per CU and
+// kWideBytes of codes for each, more where many keep the chip busy anyway. Measured
+// with it and with splits, of 128 dimensions (whole calls): 8 units of 1024 tokens
+// 11.6 and 13.5 us, of 2048 16.7 and 14.1; kernels alone: 216 units of 3500 x 64 (448
+// KB) 16.0 and 13.8 + 3.9 us, 128 of 4096 x 128 (1 MB) 42.5 and 31.0 + 4.1 us.
+constexpr uint32_t kWideWaves = 8;
 constexpr uint64_t kWideUnits = 256, kWideBytes = 256 << 10;
 // k_chunk from this many rows of a sequence and kv head on. Measured with k_step
 // and with k_chunk (bf16, 8 kv heads of 4, 128 dimensions): one sequence of 24 tokens over 8192
 // 26 and 39 us, of 256 over 2048 46 and 42, of 256 over 16384 217 and 114, of 4096 over 4096
 // 437 and 174 us; 32 of 8 tokens over 4000 84 and 133 us.
-constexpr uint64_t kChunkRows = 64;
+// At 256 dimensions, where k_chunk has one wave on a SIMD: 2 sequences of 128 rows over 4000 29
+// and 46 us, one of 592 over 1500 63 and 49.
+constexpr uint64_t chunk_from(uint32_t dim) { return dim <= 192 ? 64 : 256; }
 // Its workgroups have eight waves where that gives each CU two of them, else four:
 // 627 and 653 us for two chunks of 2048 tokens over 6000 to 10000, 42 and 36 us for
 // 1024 over 1024. Below one workgroup per CU the tokens are split, up to kChunkUnits workgroups
@@ -76,7 +77,7 @@ struct StepArgs {
   const int32_t* __restrict__ lists;  // LIST: tokens x kv_heads x count
   uint32_t count;
   float scale2;  // scale * log2(e)
-  uint32_t group, tiles, slots, splits, per;  // row tiles of a sequence (0: see tile_at), of all; 64 tokens of a split
+  uint32_t group, tiles, slots, splits, per;  // row tiles of a sequence (0: see tile_at), of all; tiles of a split
   uint16_t* __restrict__ out;
   float* __restrict__ lse;
   float* __restrict__ part;  // splits > 1: [row][split][D] sums, then [row][split][2] (R, l)
@@ -91,14 +92,17 @@ __device__ __forceinline__ float lse_of(float R, float l) {
   return l < __builtin_inff() ? ((R + e) + log2f(m)) * kLn2 : l;  // l is normal, infinite or NaN
 }
 
-constexpr int step_occ(int d) { return d <= 192 ? 2 : 1; }  // waves per SIMD, by registers
+// Tokens of a tile: what leaves the registers room for two waves on a SIMD.
+constexpr int step_tile(int d) { return d <= 192 ? 64 : 32; }
 
 template <int D, bool BF, bool LIST, bool VEC, uint32_t W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(step_occ(D), step_occ(D)))) void k_step(
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_step(
     StepArgs a) {
   constexpr int KS = D / 32;  // inner steps of the first product
   constexpr int DT = D / 16;  // row tiles of the second
   constexpr int KW = D / 16;  // words of a key row that a lane holds
+  constexpr int ST = step_tile(D) / 16;  // subtiles of 16 tokens
+  constexpr uint32_t kTile = 16 * ST, kGroup = 4 * ST;  // tokens of a tile, of a lane group
   constexpr int kPiece = KW % 4 == 0 ? 16 : 8;
   // rows 16 bytes longer than their values: 16 of them lie in different banks
   __shared__ __attribute__((aligned(16))) float sm_o[W][kRowTile][D + 4];
@@ -156,8 +160,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(step_occ
   }
   const int32_t* const table = a.b.table + (size_t)sq * a.b.width;
 
-  // this split's tiles of 64 listed tokens
-  const uint32_t all = (uint32_t)(((uint64_t)entries * bs + kTokTile - 1) / kTokTile);
+  // this split's tiles of listed tokens
+  const uint32_t all = (uint32_t)(((uint64_t)entries * bs + kTile - 1) / kTile);
   const uint32_t t_end = split + 1 < a.splits ? min(all, (split + 1) * a.per) : all;
   float* const part_ml = a.part + (size_t)a.b.tokens * a.q.heads * a.splits * D;  // splits > 1
   auto row_of = [&](uint32_t rr) {
@@ -185,7 +189,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(step_occ
   // order: to look at the last is to wait for all).
   // Lane group g has the place of its 16 tokens' block: listed (logical), then in the cache (raw).
   auto listed = [&](uint32_t tt) -> int32_t {
-    const uint32_t e = (tt * kTokTile + g * 16u) >> bsh;
+    const uint32_t e = (tt * kTile + g * kGroup) >> bsh;
     return e < entries ? LIST ? list[e] : (int32_t)e : -1;
   };
   struct Place {
@@ -194,19 +198,20 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(step_occ
   auto place = [&](uint32_t tt, int32_t lg) {
     Place p;
     p.raw = lg >= 0 && lg < seen ? table[lg] : -1;
-    p.first = (int32_t)(((uint32_t)lg << bsh) + ((tt * kTokTile + g * 16u) & (bs - 1u)));
+    p.first = (int32_t)(((uint32_t)lg << bsh) + ((tt * kTile + g * kGroup) & (bs - 1u)));
     return p;
   };
   auto block = [&](const Place& p) -> int32_t { return (uint32_t)p.raw < a.c.blocks ? p.raw : -1; };  // -1: a hole
-  uint32_t kw[4][KW];
-  u4_t vw[DT];
+  uint32_t kw[ST][KW];
+  typedef uint32_t codes_t __attribute__((ext_vector_type(ST)));
+  codes_t vw[DT];
   float ks, vs;
   auto load_keys = [&](uint32_t tt, const Place& p) {
-    const uint32_t slot = (tt * kTokTile + (n >> 2) * 16u) & (bs - 1u);
+    const uint32_t slot = (tt * kTile + (n >> 2) * kGroup) & (bs - 1u);
     const size_t cell = (size_t)max(__shfl(block(p), (int)((n >> 2) * 16u)), 0) * a.c.kvh + h;
     const int8_t* const kp = a.c.k + ((cell << bsh) + slot + (n & 3u)) * D + g * kPiece;
 #pragma unroll
-    for (int st = 0; st < 4; ++st) {
+    for (int st = 0; st < ST; ++st) {
       if constexpr (KW % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < KW / 4; ++i) {
@@ -223,11 +228,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(step_occ
     }
   };
   auto load_values = [&](uint32_t tt, const Place& p) {
-    const uint32_t slot = (tt * kTokTile + g * 16u) & (bs - 1u);
+    const uint32_t slot = (tt * kTile + g * kGroup) & (bs - 1u);
     const size_t cell = (size_t)max(block(p), 0) * a.c.kvh + h;
     const int8_t* const vp = a.c.v + ((cell * D + n) << bsh) + slot;
 #pragma unroll
-    for (int t = 0; t < DT; ++t) vw[t] = *reinterpret_cast<const u4_t*>(vp + ((size_t)(16 * t) << bsh));
+    for (int t = 0; t < DT; ++t) vw[t] = *reinterpret_cast<const codes_t*>(vp + ((size_t)(16 * t) << bsh));
   };
   auto load_scales = [&](const Place& p) {
     const float2 x = *reinterpret_cast<const float2*>(a.c.scale + ((size_t)max(block(p), 0) * a.c.kvh + h) * 2);
@@ -298,16 +303,16 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(step_occ
   q_off = rows_sum(q_off) * (-128.f * 0x1p-24f);
 
   for (; tt < t_end; tt += W) {
-    // tokens of this lane that its row sees: the first `lim` + 1 of its 16
+    // tokens of this lane that its row sees: the first `lim` + 1
     const bool hole = block(here) < 0;
     const int32_t lim = !hole && here.first <= pos ? pos - here.first : -1;
     const float y = hole ? 1.f : fmaxf(vs, kLeastScale), iv = 1.f / y;
     const float kq = fmaxf(hole ? 0.f : ks * 0x1p24f * qscale, kLeastFactor);
     const float lv = __builtin_fmaf(kq, q_off, __builtin_amdgcn_logf(y));
     const bool more = tt + W < t_end;
-    f4_t sc[4];
+    f4_t sc[ST];
 #pragma unroll
-    for (int st = 0; st < 4; ++st) {
+    for (int st = 0; st < ST; ++st) {
       sc[st] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < KS; ++c)
@@ -317,16 +322,16 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(step_occ
       load_scales(next);
       load_keys(tt + W, next);
     }
-    if (__any(lim < 15)) {
+    if (__any(lim < (int)kGroup - 1)) {
 #pragma unroll
-      for (int st = 0; st < 4; ++st)
+      for (int st = 0; st < ST; ++st)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (4 * st + i > lim) sc[st][i] = -__builtin_inff();
     }
     float most = -__builtin_inff();
 #pragma unroll
-    for (int st = 0; st < 4; ++st)
+    for (int st = 0; st < ST; ++st)
 #pragma unroll
       for (int i = 0; i < 4; ++i) most = fmaxf(most, sc[st][i]);
     const float big = __builtin_fmaf(most, kq, lv);
@@ -342,11 +347,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(step_occ
         for (int i = 0; i < 4; ++i) acc[t][i] *= f;
       R = r_new;
     }
-    h8_t pf[2];
+    h8_t pf[ST / 2];
     float add = 0.f;
     const float off = lv - R;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < ST / 2; ++u)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * u + (i >> 2)][i & 3], kq, off));
@@ -357,8 +362,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(step_occ
 #pragma unroll
     for (int t = 0; t < DT; ++t) {
       asm volatile("" : "+v"(vw[t]));  // values are waited for here, not where their conversion could begin
-      acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vw[t].x, vw[t].y), pf[0], acc[t], 0, 0, 0);
-      acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vw[t].z, vw[t].w), pf[1], acc[t], 0, 0, 0);
+#pragma unroll
+      for (int u = 0; u < ST / 2; ++u)
+        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vw[t][2 * u], vw[t][2 * u + 1]), pf[u], acc[t], 0, 0, 0);
     }
     if (more) {
       here = next;
@@ -493,7 +499,7 @@ Plan plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, bool lis
   if (b->tokens == 0) return p;
   const uint64_t group = heads / c->kv_heads;
   const uint64_t rows = list ? group : group * b->max_tokens;
-  p.chunk = !list && rows > kChunkRows;
+  p.chunk = !list && rows > chunk_from(c->dim);
   // by the rows that there are: sequences may have fewer than max_tokens
   const uint64_t big = 32 * kChunkWide;
   p.waves = c->dim <= 128 && (group * b->tokens + big - 1) / big * c->kv_heads >= kChunkUnits ? kChunkWide : kChunkSmall;
@@ -504,8 +510,9 @@ Plan plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, bool lis
   p.units = slots * c->kv_heads;
   // A split takes a fixed number of tiles, so that sequences of other lengths take
   // other numbers of workgroups.
-  const uint64_t all = ((uint64_t)(list ? count : most_blocks(c, b)) * c->block_tokens + kTokTile - 1) / kTokTile;
-  p.wide = !p.chunk && p.units <= kWideUnits && all * kTokTile * 2 * c->dim <= kWideBytes + (p.units << 10);
+  const uint64_t tokens = p.chunk ? 64 : step_tile(c->dim);  // of a tile
+  const uint64_t all = ((uint64_t)(list ? count : most_blocks(c, b)) * c->block_tokens + tokens - 1) / tokens;
+  p.wide = !p.chunk && p.units <= kWideUnits && all * tokens * 2 * c->dim <= kWideBytes + (p.units << 10);
   if (p.wide) {
     p.per = (uint32_t)all;
     p.splits = 1;
@@ -555,7 +562,6 @@ int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, c
     constexpr bool BF = decltype(bf)::value;
     auto go = [&](auto l, auto v) {
       constexpr bool L = decltype(l)::value, V = decltype(v)::value;
-      constexpr uint32_t W = wide_waves(D);
       if constexpr (!L) {
         if (p.chunk) {
           if constexpr (D <= 128) {
@@ -569,7 +575,7 @@ int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, c
         }
       }
       if (p.wide)
-        hipLaunchKernelGGL((k_step<D, BF, L, V, W>), dim3((uint32_t)grid), dim3(64 * W), 0, st, a);
+        hipLaunchKernelGGL((k_step<D, BF, L, V, kWideWaves>), dim3((uint32_t)grid), dim3(64 * kWideWaves), 0, st, a);
       else
         hipLaunchKernelGGL((k_step<D, BF, L, V, kStepWaves>), dim3((uint32_t)grid), dim3(64 * kStepWaves), 0, st, a);
     };
