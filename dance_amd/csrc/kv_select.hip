@@ -72,7 +72,7 @@ struct Codes {
   // different banks.
   static constexpr uint32_t kStride = 2 * D + 16;
   int8_t c[kRowTiles * 16 * kStride];
-  float up[kRowTiles * 16];  // 2^e of a row's codes; 0: no row
+  __attribute__((aligned(16))) float up[kRowTiles * 16];  // 2^e of a row's codes; 0: no row
   uint32_t seen[kRowTiles * 16];  // blocks that a token row sees
 };
 
@@ -207,7 +207,7 @@ __device__ __forceinline__ void score_blocks(const SelectArgs& a, const Tokens& 
       uint32_t* const at = keys + t * stride + blk;
       *at = add ? max(key, *at) : key;  // more than 16 heads: the same lane's key of those before
     };
-    auto score = [&](const Tile& b, float ks, bool hole, uint32_t blk, uint32_t r, const i4_t* qf, const float* up) {
+    auto score = [&](const Tile& b, float ks, bool hole, uint32_t blk, uint32_t r, const i4_t* qf, f4_t up) {
       i4_t acc = {0, 0, 0, 0};
 #pragma unroll
       for (int c = 0; c < KS; ++c) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf[c], b.b[c], acc, 0, 0, 0);
@@ -253,12 +253,10 @@ __device__ __forceinline__ void score_blocks(const SelectArgs& a, const Tokens& 
         turned(t0);
         for (uint32_t r = 0; r < here; ++r) {
           i4_t qf[KS];
-          float up[4];
 #pragma unroll
           for (int c = 0; c < KS; ++c)
             qf[c] = *reinterpret_cast<const i4_t*>(qc.c + (r * 16u + n) * Codes<D>::kStride + piece(c));
-#pragma unroll
-          for (int x = 0; x < 4; ++x) up[x] = qc.up[r * 16u + 4 * g + x];
+          const f4_t up = *reinterpret_cast<const f4_t*>(&qc.up[r * 16u + 4 * g]);
           score(t0, ks, hole, from + (tile + i) * 16u + n, r, qf, up);
         }
         if constexpr (kDeep) {
@@ -302,35 +300,49 @@ __device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
   };
-  // Range of the keys that compete, how many they are, and how many are forced.
+  // Four keys at a time, read before the first is looked at; a hole beyond the end.
+  constexpr uint32_t kStrip = 4;
+  auto strip = [&](uint32_t i, uint32_t step, uint32_t end, uint32_t (&k)[kStrip]) {
+#pragma unroll
+    for (uint32_t x = 0; x < kStrip; ++x) k[x] = i + x * step < end ? keys[i + x * step] : kNoKey;
+  };
+  // Range of the keys that compete, how many they are, and how many are forced. Forced
+  // keys (the largest number) wrap to 0 before the maximum, holes to the largest before the minimum.
   uint32_t lo = ~0u, hi = 0, some = 0, forced = 0;
-#pragma unroll 4
-  for (uint32_t i = tid; i < n; i += 64 * W) {
-    const uint32_t k = keys[i];
-    const bool f = k == kForced, in = k > kNoKey && !f;
-    forced += f;
-    some += in;
-    lo = min(lo, in ? k : ~0u);
-    hi = max(hi, in ? k : 0u);
+  for (uint32_t i0 = 0; i0 < n; i0 += kStrip * 64 * W) {
+    uint32_t k[kStrip];
+    strip(i0 + tid, 64 * W, n, k);
+#pragma unroll
+    for (uint32_t x = 0; x < kStrip; ++x) {
+      hi = max(hi, k[x] + 1u);
+      lo = min(lo, k[x] - (kNoKey + 1u));
+      some += (uint32_t)__popcll(__ballot(k[x] > kNoKey));
+      forced += (uint32_t)__popcll(__ballot(k[x] == kForced));
+    }
   }
-  auto reduce = [&](uint32_t lanes) {
+  auto reduce = [&](uint32_t lanes, bool counts) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       if ((uint32_t)d >= lanes) break;
       lo = min(lo, (uint32_t)__shfl_xor((int)lo, d));
       hi = max(hi, (uint32_t)__shfl_xor((int)hi, d));
-      some += (uint32_t)__shfl_xor((int)some, d);
-      forced += (uint32_t)__shfl_xor((int)forced, d);
+      if (counts) {
+        some += (uint32_t)__shfl_xor((int)some, d);
+        forced += (uint32_t)__shfl_xor((int)forced, d);
+      }
     }
   };
-  reduce(64);
+  reduce(64, false);
   if constexpr (W > 1) {
     if (lane == 0) sh.lo[wave] = lo, sh.hi[wave] = hi, sh.some[wave] = some, sh.forced[wave] = forced;
     __syncthreads();
     const uint32_t w = lane & (W - 1u);
     lo = sh.lo[w], hi = sh.hi[w], some = sh.some[w], forced = sh.forced[w];
-    reduce(W);
+    reduce(W, true);
   }
+  lo += kNoKey + 1u;
+  hi -= 1u;
+  some -= forced;
   // All keys above `limit` are taken, and the first `ties` equal to it.
   uint32_t want = less(count, forced), limit, ties = 0;
   if (some <= want) {
@@ -346,10 +358,12 @@ __device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32
         for (uint32_t i = tid; i < 256; i += 64) hist[i] = 0;
         sync();
       }
-#pragma unroll 4
-      for (uint32_t i = tid; i < n; i += 64 * W) {
-        const uint32_t k = keys[i];
-        if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> shift], 1u);
+      for (uint32_t i0 = 0; i0 < n; i0 += kStrip * 64 * W) {
+        uint32_t k[kStrip];
+        strip(i0 + tid, 64 * W, n, k);
+#pragma unroll
+        for (uint32_t x = 0; x < kStrip; ++x)
+          if (k[x] - lo <= hi - lo) atomicAdd(&hist[(k[x] - lo) >> shift], 1u);
       }
       sync();
       // lane i has counters 4 i .. 4 i + 3; counted from the largest down
@@ -393,14 +407,15 @@ __device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32
   uint32_t first = 0, rank = 0, total = 0, ranks = 0;  // taken, and equal to the limit, before this part and in all
   if constexpr (W > 1) {
     uint32_t more = 0, same = 0;
-#pragma unroll 4
-    for (uint32_t i = b0 + lane; i < b1; i += 64) {
-      const uint32_t k = keys[i];
-      more += k > limit;
-      same += k == limit;
-    }
+    for (uint32_t i0 = b0; i0 < b1; i0 += kStrip * 64) {
+      uint32_t k[kStrip];
+      strip(i0 + lane, 64, b1, k);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) more += (uint32_t)__shfl_xor((int)more, d), same += (uint32_t)__shfl_xor((int)same, d);
+      for (uint32_t x = 0; x < kStrip; ++x) {
+        more += (uint32_t)__popcll(__ballot(k[x] > limit));
+        same += (uint32_t)__popcll(__ballot(k[x] == limit && k[x] != kNoKey));
+      }
+    }
     if (lane == 0) sh.more[wave] = more, sh.same[wave] = same;
     __syncthreads();
 #pragma unroll
@@ -412,17 +427,25 @@ __device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32
   }
   uint32_t at = first;
   const uint64_t below = (1ull << lane) - 1;
-  for (uint32_t i0 = b0; i0 < b1; i0 += 64) {
-    const uint32_t i = i0 + lane;
-    const uint32_t k = i < b1 ? keys[i] : 0u;
-    const uint64_t same = __ballot(i < b1 && k == limit);
-    const uint32_t r = rank + (uint32_t)__popcll(same & below);
-    const bool take = i < b1 && (k > limit || (k == limit && r < ties));
-    const uint64_t got = __ballot(take);
-    const uint32_t pos = at + (uint32_t)__popcll(got & below);
-    if (take && pos < count) out[pos] = (int32_t)i;
-    rank += (uint32_t)__popcll(same);
-    at += (uint32_t)__popcll(got);
+  for (uint32_t i0 = b0; i0 < b1; i0 += kStrip * 64) {
+    uint32_t k[kStrip];
+    strip(i0 + lane, 64, b1, k);
+#pragma unroll
+    for (uint32_t x = 0; x < kStrip; ++x) {
+      bool take = k[x] > limit;
+      if (ties) {
+        const bool same = k[x] == limit;
+        const uint64_t mask = __ballot(same);
+        take |= same && rank + (uint32_t)__popcll(mask & below) < ties;
+        rank += (uint32_t)__popcll(mask);
+      }
+      const uint64_t got = __ballot(take);
+      if (got) {
+        const uint32_t pos = at + (uint32_t)__popcll(got & below);
+        if (take && pos < count) out[pos] = (int32_t)(i0 + lane + 64 * x);
+        at += (uint32_t)__popcll(got);
+      }
+    }
   }
   // -1 behind them
   if constexpr (W == 1) total = at;
