@@ -282,7 +282,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
       for (int i = 0; i < 8; ++i) mag = fmaxf(mag, finite_abs(load_val<true>((uint16_t)(raw[c][i >> 1] >> (16 * (i & 1))))));
     mag = rows_max(mag);
     int e = (int)(__float_as_uint(mag) >> 23) - 127 - 10;  // the largest becomes 2^10 .. 2^11
-    e = e < -100 ? -100 : e;
+    e = e < -120 ? -120 : e;  // so that the scale keeps its bits
     const float inv = exp2_int(-e);
     qscale *= exp2_int(e);
 #pragma unroll
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     const bool hole = block(here) < 0;
     const int32_t lim = !hole && here.first <= pos ? pos - here.first : -1;
     const float y = hole ? 1.f : fmaxf(vs, kLeastScale), iv = 1.f / y;
-    const float kq = fmaxf(hole ? 0.f : ks * 0x1p24f * qscale, kLeastFactor);
+    const float kq = fmaxf(hole ? 0.f : ks * qscale * 0x1p24f, kLeastFactor);
     const float lv = __builtin_fmaf(kq, q_off, __builtin_amdgcn_logf(y));
     const bool more = tt + W < t_end;
     f4_t sc[ST];
@@ -349,7 +349,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     }
     h8_t pf[ST / 2];
     float add = 0.f;
-    const float off = lv - R;
+    // lv is NaN for such queries: a row that sees none of these tokens stays as it is
+    const float off = lim < 0 ? -__builtin_inff() : lv - R;
 #pragma unroll
     for (int u = 0; u < ST / 2; ++u)
 #pragma unroll

@@ -156,7 +156,7 @@ __global__ __launch_bounds__(64 * W)
         mag = fmaxf(mag, finite_abs(load_val<true>((uint16_t)(raw[c][i >> 1] >> (16 * (i & 1))))));
     mag = half_max(mag);
     int e = (int)(__float_as_uint(mag) >> 23) - 127 - 10;
-    e = e < -100 ? -100 : e;
+    e = e < -120 ? -120 : e;  // so that the scale keeps its bits
     const float inv = exp2_int(-e);
     qscale *= exp2_int(e);
 #pragma unroll

@@ -237,8 +237,8 @@ inline const char* check_shapes(const DanceKvCache* c, const DanceKvBatch* b) {
     return "kv_heads must be in [1, 65535], blocks in [1, 2^31)";
   if (b->seqs == 0 || b->table_width == 0 || b->tokens > 0x7FFFFFFFu || b->seqs > 0x7FFFFFFFu)
     return "seqs and table_width must be positive, tokens below 2^31";
-  if ((uint64_t)b->table_width * c->block_tokens > 0x7FFFFFFFull)
-    return "a table row must hold fewer than 2^31 tokens";
+  if ((uint64_t)b->table_width * c->block_tokens > 0x7FFFFF00ull)  // positions and a tile beyond them are int32
+    return "a table row must hold at most 2^31 - 256 tokens";
   if (b->tokens && (b->max_tokens == 0 || b->max_tokens > b->tokens)) return "max_tokens must be in [1, tokens]";
   return nullptr;
 }

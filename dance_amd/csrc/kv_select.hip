@@ -213,7 +213,7 @@ __device__ __forceinline__ void score_blocks(const SelectArgs& a, const Tokens& 
       for (int c = 0; c < KS; ++c) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf[c], b.b[c], acc, 0, 0, 0);
       float x[4];  // rows 4 g + i of block n
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = up[i] > 0.f ? ((float)acc[i] * ks) * up[i] : -__builtin_inff();
+      for (int i = 0; i < 4; ++i) x[i] = up[i] > 0.f ? (float)acc[i] * (ks * up[i]) : -__builtin_inff();
       const uint32_t t0 = (p0 + r) * per_tile;
       if (a.group > 16u) {
         const float m = rows_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));

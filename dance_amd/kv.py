@@ -21,7 +21,8 @@ positions up to its own.
 
 The calls run on torch's current stream, wait for nothing and can be captured
 into a graph. As with any torch call, tensors made on another stream have to be
-ready on this one. There is no CPU path.
+ready on this one. Outputs of rows beyond the last offset are undefined. There
+are no gradients (codes are for serving) and no CPU path.
 """
 from __future__ import annotations
 

@@ -28,7 +28,8 @@
  * 0, not decreasing, none beyond `tokens`), or row b alone where offsets is
  * null (then tokens = seqs); row i of n stands at position lengths[b] - n + i
  * and sees the positions up to its own. A row at a negative position sees
- * nothing and is not written. max_tokens is at least the most rows of a
+ * nothing and is not written into the cache; the outputs of rows of no sequence
+ * (beyond the last offset) are undefined. max_tokens is at least the most rows of a
  * sequence, max_length at least the longest length (0: the table's width). */
 #ifndef DANCE_KV_H
 #define DANCE_KV_H

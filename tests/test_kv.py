@@ -415,6 +415,59 @@ def test_value_scales_of_any_ratio():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("news", [[8, 3], [90, 70]])
+def test_rows_that_see_nothing_give_zeros_whatever_their_queries(dt, news):
+    """Rows before the first token, over holes alone, or with empty lists, beside rows that see tokens."""
+    rng = np.random.default_rng(18)
+    lens = [3, 75]
+    cache, table = make(rng, 2, 128, 16, lens)
+    table[1] = -1
+    off = offsets_of(news)
+    q = torch.from_numpy(rng.normal(size=(off[-1], 4, 128))).to(dt).cuda()
+    blind = torch.tensor([i < news[0] - 3 or i >= news[0] for i in range(off[-1])], device="cuda")
+    args = dev(table), dev(np.int32(lens)), dev(off)
+    lists = np.tile(np.int32([0, -1, 4, 1]), (off[-1], 2, 1))
+    lists[news[0] - 1] = -1
+    unlisted = blind.clone()
+    unlisted[news[0] - 1] = True
+
+    def both(x):
+        return [kv.attention(cache, x, *args, max_tokens=max(news), return_lse=True),
+                kv.sparse_attention(cache, x, dev(lists), *args, max_tokens=max(news), return_lse=True)]
+    want = both(q)
+    for value in (math.nan, math.inf, -math.inf):
+        for hidden, i in ((blind, 0), (unlisted, 1)):
+            bad = q.clone()
+            bad[hidden] = value
+            bad[hidden, :, 5] = 1.0
+            o, lse = both(bad)[i]
+            assert torch.equal(o, want[i][0]) and torch.equal(lse, want[i][1])
+            assert (o[hidden] == 0).all() and torch.isneginf(lse[hidden]).all()
+
+
+@pytest.mark.gpu
+def test_large_keys_and_small_queries():
+    """Powers of two that the keys have and the queries lack change nothing, far beyond the logits' range."""
+    rng = np.random.default_rng(19)
+    lens, news = [200, 90], [3, 70]
+    cache, table = make(rng, 1, 128, 32, lens)
+    q = torch.from_numpy(rng.normal(size=(73, 2, 128))).to(BF16).cuda()
+    args = dev(table), dev(np.int32(lens))
+
+    def with_keys(e):
+        scale = cache.scale.clone()
+        scale[..., 0] *= 2.0 ** e
+        return kv.KVCache(cache.k, cache.v, scale, cache.bound)
+    for x, off in ((q[:2], None), (q, dev(offsets_of(news)))):
+        want = kv.attention(cache, x, *args, off, scale=0.1, return_lse=True)
+        got = kv.attention(with_keys(112), x * 2.0 ** -100, *args, off, scale=0.1 * 2.0 ** -12, return_lse=True)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        chosen = kv.select(with_keys(28), x, *args, 2, off)
+        assert torch.equal(chosen, kv.select(with_keys(118), x * 2.0 ** -90, *args, 2, off))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16])
 def test_rows_with_strides_and_odd_addresses(dt):
     """Queries, keys and values as slices of one projection's rows, aligned and not."""
     rng = np.random.default_rng(10)
