@@ -37,8 +37,10 @@ namespace kv {
 namespace {
 
 constexpr uint32_t kStepWaves = 4;
-constexpr uint32_t kJoinWaves = 8, kJoinRows = 4;  // waves on a row, or rows of a workgroup
-constexpr uint32_t kJoinFew = 16;                 // splits that one wave joins
+constexpr uint32_t kJoinWaves = 8;      // of k_join
+constexpr uint32_t kJoinFew = 16;       // splits that k_join_few takes
+constexpr uint32_t kJoinThreads = 256;  // of it
+constexpr uint32_t join_rows(uint32_t dim) { return kJoinThreads / (dim / 4); }
 constexpr uint32_t kRowTile = 16;
 // Waves of a workgroup that takes all of a row tile's tokens. It needs no join (and
 // its launch), but a CU reads 75 GB/s at most: up to one workgroup per CU and
@@ -421,20 +423,61 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 
 #include "kv_chunk.h"
 
-// Joins the splits of a row, one workgroup per row: the weights of up to 64
+// One row's result from its sums and their weight.
+template <bool BF>
+__device__ __forceinline__ void put_row(f4_t o, float total, uint16_t* __restrict__ out) {
+  const float inv = total > 0.f ? 1.f / total : 0.f;
+  uint16_t z[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) z[c] = store_val<BF>(total == 0.f ? 0.f : o[c] * inv);
+  *reinterpret_cast<u2_t*>(out) = u2_t{z[0] | (uint32_t)z[1] << 16, z[2] | (uint32_t)z[3] << 16};
+}
+
+// Joins a row's few splits. Every lane has four dimensions and reads all
+// splits' references itself, so that nothing is exchanged (7 ragged prompts, 12 heads of 96, 3
+// splits: 6.4 us, bound by the splits' bytes; a wave a row that exchanged them 9.1).
+template <int D, bool BF>
+__global__ __launch_bounds__(kJoinThreads) void k_join_few(const float* __restrict__ part, uint32_t splits, uint64_t rows,
+                                                           uint16_t* __restrict__ out, float* __restrict__ lse) {
+  constexpr uint32_t L = D / 4;  // lanes of a row
+  const uint64_t row = (uint64_t)blockIdx.x * join_rows(D) + threadIdx.x / L;
+  const uint32_t d = threadIdx.x % L * 4;
+  if (threadIdx.x / L >= join_rows(D) || row >= rows) return;
+  const float2* const ml = reinterpret_cast<const float2*>(part + rows * splits * D) + row * splits;
+  const float* const po = part + row * splits * D + d;
+  float m = -FLT_MAX, total = 0.f;
+  f4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (uint32_t i0 = 0; i0 < splits; i0 += 4)
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) m = fmaxf(m, ml[min(i0 + u, splits - 1u)].x);
+  for (uint32_t i0 = 0; i0 < splits; i0 += 4)
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) {
+      const uint32_t i = min(i0 + u, splits - 1u);
+      const float2 e = ml[i];
+      const float f = i0 + u < splits && e.y != 0.f ? exp2f(e.x - m) : 0.f;
+      // a split without sums was not written: the first one's line again, which is no traffic
+      const f4_t x = *reinterpret_cast<const f4_t*>(po + (size_t)(f != 0.f ? i : 0u) * D);
+      total += f != 0.f ? f * e.y : 0.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c] += f != 0.f ? f * x[c] : 0.f;
+    }
+  put_row<BF>(o, total, out + row * D + d);
+  if (lse && d == 0) lse[row] = lse_of(m, total);
+}
+
+// Joins a row's many splits, one workgroup per row: the weights of up to 64
 // splits at a time in the lanes of every wave, the sums of the splits that have
 // any shared out over the waves. (One wave per row that walked its splits took
-// 155 us for 32 rows of 256 splits.)
-template <int D, bool BF, uint32_t W>
-__global__ __launch_bounds__(64 * (W == 1 ? kJoinRows : W)) void k_join(const float* __restrict__ part, uint32_t splits,
-                                                          uint64_t rows, uint16_t* __restrict__ out,
-                                                          float* __restrict__ lse) {
+// 155 us for 32 rows of 256 splits; so 11.)
+template <int D, bool BF>
+__global__ __launch_bounds__(64 * kJoinWaves) void k_join(const float* __restrict__ part, uint32_t splits, uint64_t rows,
+                                                          uint16_t* __restrict__ out, float* __restrict__ lse) {
   constexpr uint32_t L = D / 4;  // lanes that a row of sums takes
   constexpr uint32_t P = 64 / L > 0 ? 64 / L : 1;
-  __shared__ f4_t sums[W == 1 ? kJoinRows : W][64];
-  const uint32_t lane = threadIdx.x & 63u, wave = W == 1 ? 0u : threadIdx.x >> 6;
-  const uint64_t row = W == 1 ? (uint64_t)blockIdx.x * kJoinRows + (threadIdx.x >> 6) : blockIdx.x;
-  if (W == 1 && row >= rows) return;
+  __shared__ f4_t sums[kJoinWaves][64];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint64_t row = blockIdx.x;
   const float* const ml = part + rows * splits * D + row * splits * 2;
   const float* const po = part + row * splits * D;
   float m = -FLT_MAX;
@@ -446,44 +489,33 @@ __global__ __launch_bounds__(64 * (W == 1 ? kJoinRows : W)) void k_join(const fl
   for (uint32_t i0 = 0; i0 < splits; i0 += 64) {
     const uint32_t i = i0 + lane;
     const float l = i < splits ? ml[2 * i + 1] : 0.f;
-    const float f = l != 0.f ? exp2f(ml[2 * i] - m) : 0.f;  // a split without sums was not written
+    const float f = l != 0.f ? exp2f(ml[2 * i] - m) : 0.f;
     total += f * l;
     const uint32_t n = min(64u, splits - i0);
-    auto take = [&](uint32_t k) {
+#pragma unroll
+    for (uint32_t k = wave * P; k < 64; k += kJoinWaves * P) {
+      if (k >= n) continue;
       const uint32_t at = k + lane / L;
-      const float w = __shfl(f, (int)min(at, 63u));
-      if (at < n && lane < P * L) {
-        const f4_t x = *reinterpret_cast<const f4_t*>(po + (size_t)(i0 + at) * D + lane % L * 4);
+      const float other = __shfl(f, (int)min(at, 63u)), w = at < 64u && lane < P * L ? other : 0.f;
+      // without sums: the first split's line again, as above
+      const f4_t x = *reinterpret_cast<const f4_t*>(po + (size_t)(w != 0.f ? i0 + at : 0u) * D + lane % L * 4);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] += w != 0.f ? w * x[c] : 0.f;
-      }
-    };
-    if constexpr (W == 1) {
-      for (uint32_t k = 0; k < n; k += P) take(k);
-    } else {
-#pragma unroll
-      for (uint32_t k = wave * P; k < 64; k += W * P)
-        if (k < n) take(k);
+      for (int c = 0; c < 4; ++c) o[c] += w != 0.f ? w * x[c] : 0.f;
     }
   }
 #pragma unroll
   for (int x = 1; x < 64; x <<= 1) total += __shfl_xor(total, x);
-  f4_t* const mine = sums[W == 1 ? threadIdx.x >> 6 : 0];  // W == 1: the wave's own, in program order
-  sums[threadIdx.x >> 6][lane] = o;
-  if constexpr (W > 1) __syncthreads();
+  sums[wave][lane] = o;
+  __syncthreads();
   if (wave == 0 && lane < L) {
     f4_t y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (uint32_t w = 0; w < W; ++w)
+    for (uint32_t w = 0; w < kJoinWaves; ++w)
 #pragma unroll
       for (uint32_t p = 0; p < P; ++p)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) y[c] += mine[w * 64 + p * L + lane][c];
-    const float inv = total > 0.f ? 1.f / total : 0.f;
-    uint16_t z[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) z[c] = store_val<BF>(total == 0.f ? 0.f : y[c] * inv);
-    *reinterpret_cast<u2_t*>(out + row * D + lane * 4) = u2_t{z[0] | (uint32_t)z[1] << 16, z[2] | (uint32_t)z[3] << 16};
+        for (int c = 0; c < 4; ++c) y[c] += sums[w][p * L + lane][c];
+    put_row<BF>(y, total, out + row * D + lane * 4);
     if (lse && lane == 0) lse[row] = lse_of(m, total);
   }
 }
@@ -586,11 +618,11 @@ int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, c
       vec ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
     const uint64_t rows = (uint64_t)batch->tokens * q->heads;
     if (p.splits > kJoinFew)
-      hipLaunchKernelGGL((k_join<D, BF, kJoinWaves>), dim3((uint32_t)rows), dim3(64 * kJoinWaves), 0, st, a.part,
-                         p.splits, rows, a.out, lse);
+      hipLaunchKernelGGL((k_join<D, BF>), dim3((uint32_t)rows), dim3(64 * kJoinWaves), 0, st, a.part, p.splits, rows,
+                         a.out, lse);
     else if (p.splits > 1)
-      hipLaunchKernelGGL((k_join<D, BF, 1>), dim3((uint32_t)((rows + kJoinRows - 1) / kJoinRows)),
-                         dim3(64 * kJoinRows), 0, st, a.part, p.splits, rows, a.out, lse);
+      hipLaunchKernelGGL((k_join_few<D, BF>), dim3((uint32_t)((rows + join_rows(D) - 1) / join_rows(D))),
+                         dim3(kJoinThreads), 0, st, a.part, p.splits, rows, a.out, lse);
   });
   return launched(who);
 }
