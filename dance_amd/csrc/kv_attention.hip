@@ -25,6 +25,13 @@
 // 2^(kLift + kSlack), inside f16, which rounds it to 11 bits (down to 2^-27 of a row's largest; the
 // f16 outputs have 11 bits too). l and all sums are float32, l of unrounded
 // p. Scales below 2^kLeastExp count as that, so that 1 / y is finite.
+//
+// Bound by the codes' bytes: a step reads each once and does 4 operations on it per row. Measured (8 kv
+// heads of 4, 128 dimensions): 64 sequences of 500 to 12,000 tokens, 497 MB, 104 us (4.8 TB/s, a large copy's rate);
+// 2 of 400,000 to 600,000, 461 MB, 85 us (5.4 TB/s) and 11 of join; 16 rows over 64 listed blocks
+// of 64 tokens each, 135 MB, 27 us (5.0 TB/s). One sequence of 700 tokens takes 9.6 us, a chain of dependent loads.
+// Lists of 1026 rows over the same 145 MB are bound by instructions (64 % of the cycles) and by
+// what the L2s miss of them (1.4 GB): 301 us.
 
 #include <cfloat>
 #include <cmath>
