@@ -290,6 +290,42 @@ __device__ __forceinline__ void clear_teams(Team* tm) {
   for (uint32_t i = threadIdx.x; i < kRounds * 256; i += kSelThreads) tm[i >> 8].hist[i & 255u] = 0;
 }
 
+// Without LDS: over the 16 lanes that differ in bits 0 to 3, then over all 64.
+template <typename Op>
+__device__ __forceinline__ uint32_t over16(uint32_t x, Op op) {
+  auto with = [&](auto ctrl) {  // as in cols_max
+    x = op(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  with(Int<0xB1>{});
+  with(Int<0x4E>{});
+  with(Int<0x141>{});
+  with(Int<0x140>{});
+  return x;
+}
+template <typename Op>
+__device__ __forceinline__ uint32_t over64(uint32_t x, Op op) {
+  x = over16(x, op);
+  const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  x = op(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)op(b[0], b[1]));
+}
+// Sum over this lane and those after it: within rows of 16 by shifts, then the rows behind.
+__device__ __forceinline__ uint32_t sum_from(uint32_t x) {
+  auto with = [&](auto ctrl) {  // lane i + 1, 2, 4, 8 of the row; 0 beyond its end
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xF, 0xF, true);
+  };
+  with(Int<0x101>{});
+  with(Int<0x102>{});
+  with(Int<0x104>{});
+  with(Int<0x108>{});
+  const uint32_t r3 = (uint32_t)__builtin_amdgcn_readlane((int)x, 48);
+  const uint32_t r2 = r3 + (uint32_t)__builtin_amdgcn_readlane((int)x, 32);
+  const uint32_t r1 = r2 + (uint32_t)__builtin_amdgcn_readlane((int)x, 16);
+  const uint32_t row = (threadIdx.x & 63u) >> 4;
+  return x + (row == 0 ? r1 : row == 1 ? r2 : row == 2 ? r3 : 0u);
+}
+
 // The `count` blocks of the n with the largest keys, ties to the lower block, ascending.
 template <uint32_t W>
 __device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32_t n, uint32_t count,
@@ -325,25 +361,21 @@ __device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32
       forced += (uint32_t)__popcll(__ballot(k[x] == kForced));
     }
   }
-  auto reduce = [&](uint32_t lanes, bool counts) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      if ((uint32_t)d >= lanes) break;
-      lo = min(lo, (uint32_t)__shfl_xor((int)lo, d));
-      hi = max(hi, (uint32_t)__shfl_xor((int)hi, d));
-      if (counts) {
-        some += (uint32_t)__shfl_xor((int)some, d);
-        forced += (uint32_t)__shfl_xor((int)forced, d);
-      }
-    }
-  };
-  reduce(64, false);
+  auto least = [](uint32_t a, uint32_t b) { return min(a, b); };
+  auto most = [](uint32_t a, uint32_t b) { return max(a, b); };
+  auto sum = [](uint32_t a, uint32_t b) { return a + b; };
+  auto same_in_all = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
+  lo = over64(lo, least);
+  hi = over64(hi, most);
   if constexpr (W > 1) {
+    static_assert(W == 16, "over16");
     if (lane == 0) sh.lo[wave] = lo, sh.hi[wave] = hi, sh.some[wave] = some, sh.forced[wave] = forced;
     __syncthreads();
     const uint32_t w = lane & (W - 1u);
-    lo = sh.lo[w], hi = sh.hi[w], some = sh.some[w], forced = sh.forced[w];
-    reduce(W, true);
+    lo = same_in_all(over16(sh.lo[w], least));
+    hi = same_in_all(over16(sh.hi[w], most));
+    some = same_in_all(over16(sh.some[w], sum));
+    forced = same_in_all(over16(sh.forced[w], sum));
   }
   lo += kNoKey + 1u;
   hi -= 1u;
@@ -375,12 +407,7 @@ __device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32
       uint32_t c[4], mine = 0;
 #pragma unroll
       for (int x = 0; x < 4; ++x) c[x] = hist[4 * lane + x], mine += c[x];
-      uint32_t from = mine;  // over this lane and those after it
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = (uint32_t)__shfl_down((int)from, d);
-        if (lane + d < 64) from += o;
-      }
+      const uint32_t from = sum_from(mine);
       uint32_t above = from - mine;
       const bool here = above < want && from >= want;
       uint32_t digit = 0, left = 0, full = 0;
@@ -390,10 +417,10 @@ __device__ __forceinline__ void choose(const uint32_t* __restrict__ keys, uint32
         above += c[x];
       }
       const int src = __ffsll((unsigned long long)__ballot(here)) - 1;
-      digit = (uint32_t)__shfl((int)digit, src);
-      want = (uint32_t)__shfl((int)left, src);
+      digit = (uint32_t)__builtin_amdgcn_readlane((int)digit, src);
+      want = (uint32_t)__builtin_amdgcn_readlane((int)left, src);
       lo += digit << shift;
-      if (__shfl((int)full, src)) {  // all of this counter's keys
+      if (__builtin_amdgcn_readlane((int)full, src)) {  // all of this counter's keys
         limit = lo - 1u;
         break;
       }
