@@ -77,7 +77,7 @@ struct Codes {
   // different banks.
   static constexpr uint32_t kStride = 2 * D + 16;
   int8_t c[kRowTiles * 16 * kStride];
-  __attribute__((aligned(16))) float up[kRowTiles * 16];  // 2^e of a row's codes; 0: no row
+  __attribute__((aligned(16))) float up[kRowTiles * 16];  // 2^e of a row's codes
   uint32_t seen[kRowTiles * 16];  // blocks that a token row sees
 };
 
@@ -90,10 +90,10 @@ __device__ __forceinline__ void code_rows(const SelectArgs& a, const Tokens& tk,
   const uint32_t end = min((uint32_t)kRowTiles, rows - p0) * 16u;
   for (uint32_t r = threadIdx.x >> 4; r < end; r += kSelThreads / 16) {
     const uint32_t t = a.group > 16u ? 0u : (p0 * 16u + r) / a.gp;
-    const uint32_t f = a.group > 16u ? p0 * 16u + r : r % a.gp;
-    const bool live = t < tk.n && f < a.group;
-    const uint16_t* const src = a.q.data + (int64_t)(tk.row + (live ? t : 0u)) * a.q.token_stride +
-                                (int64_t)(h * a.group + (live ? f : 0u)) * a.q.head_stride + l * V;
+    // rows of no head repeat the group's last, which changes no maximum; those of no token are not used
+    const uint32_t f = min(a.group > 16u ? p0 * 16u + r : r % a.gp, a.group - 1u);
+    const uint16_t* const src = a.q.data + (int64_t)(tk.row + min(t, tk.n - 1u)) * a.q.token_stride +
+                                (int64_t)(h * a.group + f) * a.q.head_stride + l * V;
     float x[V];
     if constexpr (VEC && V % 4 == 0) {
 #pragma unroll
@@ -119,7 +119,7 @@ __device__ __forceinline__ void code_rows(const SelectArgs& a, const Tokens& tk,
       out[i] = (int8_t)max(code, 0);
       out[D + i] = (int8_t)min(code, 0);
     }
-    if (l == 0) qc.up[r] = live ? exp2_int(e) : 0.f;
+    if (l == 0) qc.up[r] = exp2_int(e);
   }
 }
 
@@ -218,7 +218,7 @@ __device__ __forceinline__ void score_blocks(const SelectArgs& a, const Tokens& 
       for (int c = 0; c < KS; ++c) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf[c], b.b[c], acc, 0, 0, 0);
       float x[4];  // rows 4 g + i of block n
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = up[i] > 0.f ? (float)acc[i] * (ks * up[i]) : -__builtin_inff();
+      for (int i = 0; i < 4; ++i) x[i] = (float)acc[i] * (ks * up[i]);
       const uint32_t t0 = (p0 + r) * per_tile;
       if (a.group > 16u) {
         const float m = rows_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
