@@ -17,10 +17,10 @@
 // count-th largest until it is all taken or a single key, and writes what
 // is larger, and of what equals it the first ones, in index order.
 //
-// Measured (8 kv heads of 4, 128 dimensions): 16 rows over 60,000 to 131,072 tokens in blocks of 64, 52 MB, 25 us,
-// a workgroup's loads and lane exchange of 2048 blocks, then 8 of choice; 1026 rows of two
-// sequences over 20,000 to 40,000 in blocks of 32, 72 us, of which the choice 35, loads and exchange 25,
-// products and keys 22 (they overlap), all bound by LDS and vector instructions.
+// Measured (8 kv heads of 4, 128 dimensions): 16 rows over 60,000 to 131,072 tokens in blocks of 64, 52 MB, 23 us,
+// a workgroup's loads and lane exchange of 2048 blocks, then 6 of choice; 1026 rows of two
+// sequences over 20,000 to 40,000 in blocks of 32, 71 us, of which the choice 32, loads and exchange 25,
+// products and keys 20 (they overlap), all bound by LDS and vector instructions.
 
 #include <cmath>
 #include <type_traits>
