@@ -24,7 +24,10 @@
 // row that stays until s + log2 y exceeds it by kLift + kSlack: p is then at most
 // 2^(kLift + kSlack), inside f16, which rounds it to 11 bits (down to 2^-27 of a row's largest; the
 // f16 outputs have 11 bits too). l and all sums are float32, l of unrounded
-// p. Scales below 2^kLeastExp count as that, so that 1 / y is finite.
+// p. Scales below 2^kLeastExp count as that, so that 1 / y is finite. l is held in units of 1 /
+// kSumUnit: where all values are zero or of the least scale a token adds up to 2^(15 + 100) to it, and a
+// table row's 2^31 tokens stay below 2^128. A token of such a block beside blocks of larger values counts in
+// l where its weight is more than 2^-41 times their scale of theirs (p is then a normal number).
 //
 // Bound by the codes' bytes: a step reads each once and does 4 operations on it per row. Measured (8 kv
 // heads of 4, 128 dimensions): 64 sequences of 500 to 12,000 tokens, 497 MB, 104 us (4.8 TB/s, a large copy's rate);
@@ -75,6 +78,7 @@ constexpr float kLift = 13.f, kSlack = 2.f;
 constexpr float kLeastScale = 0x1p-100f;  // 2^kLeastExp
 // Least factor of a product: above 0, so that a hidden token's, -infinity, stays that.
 constexpr float kLeastFactor = 0x1p-120f;
+constexpr float kSumUnit = 0x1p-20f;  // of l, see above
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kSplitUnits = 1024;  // workgroups that fill the chip several times over
 constexpr uint32_t kSplitTiles = 16;    // least tiles of a split: its partial sums are then 2 to 6 % of what it reads
@@ -92,13 +96,43 @@ struct StepArgs {
   float* __restrict__ part;  // splits > 1: [row][split][D] sums, then [row][split][2] (R, l)
 };
 
-// ln(l 2^R). R and the exponent of l are of opposite signs and about one size: their sum
+// A sum of many tiles with what its additions rounded off: without it the logarithm of 140,000
+// tokens' sum is off by 2e-5 where a wave walks them all.
+struct Sum {
+  float x = 0.f, low = 0.f;
+  __device__ __forceinline__ void add(float y) {
+    y -= low;
+    const float t = x + y;
+    low = (t - x) - y;
+    x = t;
+  }
+  __device__ __forceinline__ void scale(float f) {
+    x *= f;
+    low *= f;
+  }
+};
+
+// ln(l 2^R / kSumUnit). R and the exponent of l are of opposite signs and about one size: their sum
 // first, or the logarithm's rounding is that of the larger number.
 __device__ __forceinline__ float lse_of(float R, float l) {
   if (l == 0.f) return -__builtin_inff();
-  const uint32_t u = __float_as_uint(l);
-  const float e = (float)((int)(u >> 23) - 127), m = __uint_as_float((u & 0x7FFFFFu) | 0x3F800000u);
-  return l < __builtin_inff() ? ((R + e) + log2f(m)) * kLn2 : l;  // l is normal, infinite or NaN
+  const bool small = l < 1.f;  // perhaps subnormal in its unit
+  const uint32_t u = __float_as_uint(small ? l * (1.f / kSumUnit) : l);
+  const float e = (float)((int)(u >> 23) - (small ? 127 : 107)), m = __uint_as_float((u & 0x7FFFFFu) | 0x3F800000u);
+  return l < __builtin_inff() ? ((R + e) + log2f(m)) * kLn2 : l;  // l is finite, infinite or NaN
+}
+static_assert(kSumUnit == 0x1p-20f, "lse_of's exponents");
+
+// Four of a row's sums over l, as the output's type; zeros where nothing was summed. The
+// unit goes to the factor that it leaves normal.
+template <bool BF>
+__device__ __forceinline__ u2_t quotients(f4_t o, float l) {
+  const bool small = l < 1.f;
+  const float unit = small ? 1.f : kSumUnit, inv = l > 0.f ? 1.f / (small ? l * (1.f / kSumUnit) : l) : 0.f;
+  uint16_t y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = store_val<BF>(l == 0.f ? 0.f : o[i] * unit * inv);
+  return u2_t{y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16};
 }
 
 // Tokens of a tile: what leaves the registers room for two waves on a SIMD.
@@ -189,7 +223,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   f4_t acc[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) acc[t] = f4_t{0.f, 0.f, 0.f, 0.f};
-  float R = -FLT_MAX, l = 0.f;
+  float R = -FLT_MAX;
+  Sum l;
 
   // Loads run ahead in the registers that the products have read: the next
   // tile's keys set out behind the first product, its values behind the second, the
@@ -349,7 +384,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
       const float row_big = rows_max(big);
       const float r_new = row_big > R + (kLift + kSlack) ? row_big - kLift : R;
       const float f = exp2f(R - r_new);
-      l *= f;
+      l.scale(f);
 #pragma unroll
       for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -368,7 +403,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         add += p;
         pf[u][i] = (_Float16)p;
       }
-    l += add * iv;
+    l.add(add * iv * kSumUnit);
 #pragma unroll
     for (int t = 0; t < DT; ++t) {
       asm volatile("" : "+v"(vw[t]));  // values are waited for here, not where their conversion could begin
@@ -385,10 +420,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   }
 
   // The waves' sums meet in LDS, in wave order.
-  l = rows_sum(l);
+  const float sum_l = rows_sum(l.x);
   if (g == 0) {
     sm_m[wave][n] = R;
-    sm_l[wave][n] = l;
+    sm_l[wave][n] = sum_l;
   }
   if (n < rows)
 #pragma unroll
@@ -418,27 +453,13 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         pm[1] = sum;
       }
     } else {
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
-      uint16_t y[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) y[x] = store_val<BF>(sum == 0.f ? 0.f : o[x] * inv);
-      *reinterpret_cast<u2_t*>(a.out + row * D + d) = u2_t{y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16};
+      *reinterpret_cast<u2_t*>(a.out + row * D + d) = quotients<BF>(o, sum);
       if (a.lse && d == 0) a.lse[row] = lse_of(m, sum);
     }
   }
 }
 
 #include "kv_chunk.h"
-
-// One row's result from its sums and their weight.
-template <bool BF>
-__device__ __forceinline__ void put_row(f4_t o, float total, uint16_t* __restrict__ out) {
-  const float inv = total > 0.f ? 1.f / total : 0.f;
-  uint16_t z[4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) z[c] = store_val<BF>(total == 0.f ? 0.f : o[c] * inv);
-  *reinterpret_cast<u2_t*>(out) = u2_t{z[0] | (uint32_t)z[1] << 16, z[2] | (uint32_t)z[3] << 16};
-}
 
 // Joins a row's few splits. Every lane has four dimensions and reads all
 // splits' references itself, so that nothing is exchanged (7 ragged prompts, 12 heads of 96, 3
@@ -469,7 +490,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_join_few(const float* __restri
 #pragma unroll
       for (int c = 0; c < 4; ++c) o[c] += f != 0.f ? f * x[c] : 0.f;
     }
-  put_row<BF>(o, total, out + row * D + d);
+  *reinterpret_cast<u2_t*>(out + row * D + d) = quotients<BF>(o, total);
   if (lse && d == 0) lse[row] = lse_of(m, total);
 }
 
@@ -522,7 +543,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_join(const float* __restric
       for (uint32_t p = 0; p < P; ++p)
 #pragma unroll
         for (int c = 0; c < 4; ++c) y[c] += sums[w][p * L + lane][c];
-    put_row<BF>(y, total, out + row * D + lane * 4);
+    *reinterpret_cast<u2_t*>(out + row * D + lane * 4) = quotients<BF>(y, total);
     if (lse && lane == 0) lse[row] = lse_of(m, total);
   }
 }

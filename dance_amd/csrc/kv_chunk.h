@@ -179,7 +179,8 @@ __global__ __launch_bounds__(64 * W)
   const int32_t p_most = idle ? -1 : pos_of(r_first + min(w_first + 32u, rows) - 1u);
 
   f16_t acc[DT];
-  float R = -FLT_MAX, l = 0.f;
+  float R = -FLT_MAX;
+  Sum l;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -240,13 +241,14 @@ __global__ __launch_bounds__(64 * W)
         const float row_big = half_max(big);
         const float r_new = row_big > R + (kLift + kSlack) ? row_big - kLift : R;
         const float f = exp2f(R - r_new);
-        l *= f;
+        l.scale(f);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[d][i] *= f;
         R = r_new;
       }
+      float part = 0.f;  // at most 2^120: 32 tokens of the least scale
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float c = grp[j].y - R;
@@ -258,8 +260,9 @@ __global__ __launch_bounds__(64 * W)
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) pf[j][i] = (_Float16)p[i];
-        l = __builtin_fmaf(add, grp[j].z, l);
+        part = __builtin_fmaf(add, grp[j].z, part);
       }
+      l.add(part * kSumUnit);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -277,7 +280,7 @@ __global__ __launch_bounds__(64 * W)
     }
   }
 
-  const float sum = half_sum(l);
+  const float sum = half_sum(l.x);
   const uint32_t rr = wave * 32u + n;
   if (rr >= rows) return;
   const size_t row = row_of(rr);
@@ -295,17 +298,13 @@ __global__ __launch_bounds__(64 * W)
       pm[1] = sum;
     }
   } else {
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
     uint16_t* const out = a.out + row * D + 4 * hl;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        uint16_t y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = store_val<BF>(sum == 0.f ? 0.f : acc[d][4 * x + i] * inv);
-        *reinterpret_cast<u2_t*>(out + 32 * d + 8 * x) = u2_t{y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16};
-      }
+      for (int x = 0; x < 4; ++x)
+        *reinterpret_cast<u2_t*>(out + 32 * d + 8 * x) =
+            quotients<BF>(f4_t{acc[d][4 * x], acc[d][4 * x + 1], acc[d][4 * x + 2], acc[d][4 * x + 3]}, sum);
     if (a.lse && hl == 0) a.lse[row] = lse_of(R, sum);
   }
 }
