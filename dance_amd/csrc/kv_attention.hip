@@ -589,13 +589,17 @@ Plan plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, bool lis
   return p;
 }
 
+bool count_fits(const DanceKvCache* c, uint32_t count) {
+  return count != 0 && (uint64_t)count * c->block_tokens <= 0x7FFFFFFFull;
+}
+
 int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, const DanceKvRows* q,
         const int32_t* lists, bool list, uint32_t count, float scale, void* out, float* lse, void* work,
         size_t work_bytes, void* stream) {
   const char* why = check_common(cache, batch);
   if (!why) why = check_rows(cache, q, false);
   if (!why && (!out || !aligned(out, 16))) why = "out must be given, aligned to 16 bytes";
-  if (!why && list && (!lists || count == 0 || (uint64_t)count * cache->block_tokens > 0x7FFFFFFFull))
+  if (!why && list && (!lists || !count_fits(cache, count)))
     why = "lists must be given, with 1 to 2^31 / block_tokens entries";
   if (!why && !(scale == scale && std::fabs(scale) < INFINITY)) why = "scale must be finite";
   if (why) {
@@ -682,7 +686,7 @@ int dance_kv_sparse_attention(const DanceKvCache* cache, const DanceKvBatch* bat
 
 size_t dance_kv_sparse_attention_work(const DanceKvCache* cache, const DanceKvBatch* batch, uint32_t heads,
                                       uint32_t count) {
-  if (check_shapes(cache, batch) || heads == 0 || heads % cache->kv_heads) return 0;
+  if (check_shapes(cache, batch) || heads == 0 || heads % cache->kv_heads || !count_fits(cache, count)) return 0;
   return plan(cache, batch, heads, true, count).work;
 }
 

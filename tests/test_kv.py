@@ -746,6 +746,14 @@ def test_entries_refuse_what_else_is_missing(capfd):
         assert need > 0 and L.dance_kv_select(c, b, r, 4, 0, 0, 1 << 20, at, size, None) == -1
 
 
+def test_workspaces_of_lists_that_the_call_refuses():
+    L = kv._bind()
+    c, b, _ = fake(kv_heads=8, seqs=64, tokens=64, max_tokens=1, offsets=None)
+    assert L.dance_kv_sparse_attention_work(c, b, 32, 1 << 20) > 0
+    assert L.dance_kv_sparse_attention_work(c, b, 32, 0) == 0  # 512 units: more than one launch rule's 256
+    assert L.dance_kv_sparse_attention_work(c, b, 32, 1 << 27) == 0
+
+
 def test_library_exports_every_declared_entry():
     text = open(D.HERE + "/../include/dance_kv.h").read()
     names = set(re.findall(r"\b(dance_kv_\w+)\(const", text))
