@@ -274,7 +274,7 @@ inline bool rows_vector(const DanceKvRows* r) {
 }
 // Blocks of a sequence that a call may meet.
 inline uint32_t most_blocks(const DanceKvCache* c, const DanceKvBatch* b) {
-  const uint64_t n = b->max_length ? (b->max_length + c->block_tokens - 1) / c->block_tokens : b->table_width;
+  const uint64_t n = b->max_length ? (b->max_length - 1) / c->block_tokens + 1 : b->table_width;
   return n < b->table_width ? (uint32_t)n : b->table_width;
 }
 

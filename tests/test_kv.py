@@ -754,6 +754,15 @@ def test_workspaces_of_lists_that_the_call_refuses():
     assert L.dance_kv_sparse_attention_work(c, b, 32, 1 << 27) == 0
 
 
+def test_a_longest_length_beyond_the_table_counts_as_the_table():
+    L = kv._bind()
+    for longest in (0, 5000 * 16, 1 << 40, (1 << 64) - 1):
+        c, b, _ = fake(seqs=1, tokens=1, max_tokens=1, offsets=None, table_width=5000, max_length=longest)
+        assert [L.dance_kv_attention_work(c, b, 4), L.dance_kv_select_work(c, b, 4, 8)] == [4 * 79 * 66 * 4, 2 * 5000 * 4]
+    c, b, _ = fake(seqs=200, tokens=200, max_tokens=1, offsets=None, table_width=5000, max_length=(1 << 64) - 1)
+    assert L.dance_kv_attention_work(c, b, 4) == 200 * 4 * 3 * 66 * 4  # 400 units: not one workgroup each
+
+
 def test_library_exports_every_declared_entry():
     text = open(D.HERE + "/../include/dance_kv.h").read()
     names = set(re.findall(r"\b(dance_kv_\w+)\(const", text))
