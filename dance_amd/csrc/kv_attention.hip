@@ -612,8 +612,12 @@ int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, c
     std::fprintf(stderr, "[%s] work must hold %zu bytes, aligned to 16\n", who, p.work);
     return -1;
   }
-  const uint64_t grid = p.units * p.splits;
-  if (grid * 64 * 8 > 0xFFFFFFFFull || (uint64_t)batch->tokens * q->heads * 64 * kJoinWaves > 0xFFFFFFFFull) {
+  // Rows are counted in 31 bits, a launch's threads in 32; the joins' grids count where there is a join.
+  const uint64_t grid = p.units * p.splits, rows = (uint64_t)batch->tokens * q->heads;
+  const uint64_t join = p.splits > kJoinFew ? rows * 64 * kJoinWaves
+                        : p.splits > 1      ? (rows / join_rows(cache->dim) + 1) * kJoinThreads
+                                            : 0;
+  if (grid * 64 * 8 > 0xFFFFFFFFull || rows > 0x7FFFFFFFull || join > 0xFFFFFFFFull) {
     std::fprintf(stderr, "[%s] batch is too large for one launch\n", who);
     return -1;
   }
@@ -648,7 +652,6 @@ int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, c
       vec ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
     else
       vec ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
-    const uint64_t rows = (uint64_t)batch->tokens * q->heads;
     if (p.splits > kJoinFew)
       hipLaunchKernelGGL((k_join<D, BF>), dim3((uint32_t)rows), dim3(64 * kJoinWaves), 0, st, a.part, p.splits, rows,
                          a.out, lse);

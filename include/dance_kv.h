@@ -30,7 +30,10 @@
  * and sees the positions up to its own. A row at a negative position sees
  * nothing and is not written into the cache; the outputs of rows of no sequence
  * (beyond the last offset) are undefined. max_tokens is at least the most rows of a
- * sequence, max_length at least the longest length (0: the table's width). */
+ * sequence, max_length at least the longest length (0: the table's width).
+ * A call is one launch of fewer than 2^32 threads (and a join of splits, where there are any), and refuses a batch that
+ * needs more: attention has room for 2^23 single rows x kv heads (of up to 16 heads each), and for prompts of
+ * some 2^30 rows x heads. */
 #ifndef DANCE_KV_H
 #define DANCE_KV_H
 

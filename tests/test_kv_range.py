@@ -1,11 +1,13 @@
 """The key-value cache operators at the ends of their ranges: values and scales, numbers of
 tokens, and the kernels that only large calls reach. Definitions and tolerances: test_kv.py."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
 from dance_amd import kv
-from test_kv import BF16, Model, check_attention, dev, make, numbers, offsets_of
+from test_kv import BF16, Model, check_attention, dev, fake, make, numbers, offsets_of
 
 # tokens over which a block repeats, sequences, rows of each, block tokens and dim: what joins the sums
 LONG = [
@@ -65,3 +67,35 @@ def test_values_of_the_least_and_the_largest_scales(e, rows):
     q = torch.from_numpy(rng.normal(size=(off[-1], 4, 128))).to(BF16).cuda()
     got, lse = kv.attention(cache, q, dev(table), dev(np.int32(lens)), dev(off), max_tokens=rows, return_lse=True)
     check_attention(Model(cache), got, lse, q, table, lens, off, 128 ** -0.5)
+
+@pytest.mark.gpu
+def test_prompt_of_more_rows_than_a_join_takes():
+    """131,072 tokens of 64 heads, 2^23 rows: nothing is joined, so that only the kernel's own grid counts."""
+    rng = np.random.default_rng(23)
+    n, heads, dim, bs = 131072, 64, 64, 16
+    cache, table = make(rng, 1, dim, bs, [bs])
+    at = table[0, 0]
+    g = torch.Generator(device="cuda").manual_seed(23)
+    q = torch.randn((n, heads, dim), generator=g, device="cuda").to(BF16)
+    got, lse = kv.attention(cache, q, dev(table[:, :1]), dev(np.int32([n])), dev(np.int32([0, n])), return_lse=True)
+    keys = cache.k[at, 0].double() * cache.scale[at, 0, 0]
+    vals = (cache.v[at, 0].double() * cache.scale[at, 0, 1]).t().contiguous()
+    step = 8192
+    for t in range(0, n, step):
+        x = q[t:t + step].double().view(-1, dim)
+        logits = x @ keys.t().contiguous() * dim ** -0.5
+        pos = torch.arange(t, t + step, device="cuda").repeat_interleave(heads)
+        logits.masked_fill_(torch.arange(bs, device="cuda") > pos[:, None], -math.inf)
+        want = torch.logsumexp(logits, 1)
+        p = torch.exp(logits - want[:, None])
+        d = (x.abs() @ keys.abs().t().contiguous()).amax(1) * dim ** -0.5 * (dim + 8) * 2.0 ** -24
+        o, absolute = p @ vals, p @ vals.abs()
+        tol = 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2 * d[:, None] + 2.0 ** -18) * absolute
+        assert ((got[t:t + step].double().view(-1, dim) - o).abs() <= tol).all()
+        assert ((lse[t:t + step].double().view(-1) - want).abs() <= d + 2.0 ** -20 * (1 + want.abs())).all()
+
+
+def test_batches_too_large_for_a_launch_are_refused(capfd):
+    c, b, r = fake(seqs=1, tokens=1 << 30, max_tokens=1 << 30, table_width=1)
+    assert kv._bind().dance_kv_attention(c, b, r, 1.0, 1 << 20, None, 1 << 20, 1 << 60, None) == -1
+    assert "too large for one launch" in capfd.readouterr().err
