@@ -338,21 +338,14 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 #pragma unroll
     for (int c = 0; c < KS; ++c) qf[c] = __builtin_bit_cast(h8_t, raw[c] ^ u4_t{flip, flip, flip, flip});
   }
-  // What the key operand has too much, 128 for each code (small8), in its products.
-  float q_off = 0.f;
-#pragma unroll
-  for (int c = 0; c < KS; ++c)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q_off += (float)qf[c][i];
-  q_off = rows_sum(q_off) * (-128.f * 0x1p-24f);
 
   for (; tt < t_end; tt += W) {
     // tokens of this lane that its row sees: the first `lim` + 1
     const bool hole = block(here) < 0;
     const int32_t lim = !hole && here.first <= pos ? pos - here.first : -1;
     const float y = hole ? 1.f : fmaxf(vs, kLeastScale), iv = 1.f / y;
-    const float kq = fmaxf(hole ? 0.f : ks * qscale * 0x1p24f, kLeastFactor);
-    const float lv = __builtin_fmaf(kq, q_off, __builtin_amdgcn_logf(y));
+    const float kq = fmaxf(hole ? 0.f : ks * qscale, kLeastFactor);
+    const float lv = __builtin_amdgcn_logf(y);
     const bool more = tt + W < t_end;
     f4_t sc[ST];
 #pragma unroll
@@ -360,7 +353,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
       sc[st] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < KS; ++c)
-        sc[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(small8(kw[st][2 * c], kw[st][2 * c + 1]), qf[c], sc[st], 0, 0, 0);
+        sc[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(kw[st][2 * c], kw[st][2 * c + 1]), qf[c], sc[st], 0, 0, 0);
     }
     if (more) {
       load_scales(next);
@@ -393,8 +386,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     }
     h8_t pf[ST / 2];
     float add = 0.f;
-    // lv is NaN for such queries: a row that sees none of these tokens stays as it is
-    const float off = lim < 0 ? -__builtin_inff() : lv - R;
+    const float off = lv - R;
 #pragma unroll
     for (int u = 0; u < ST / 2; ++u)
 #pragma unroll

@@ -171,17 +171,6 @@ __device__ __forceinline__ h8_t codes8(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(h8_t, u4_t{x.x, x.y, y.x, y.y});
 }
 
-// Eight codes as (c + 128) * 2^-24, f16 subnormals, which the MFMAs take as they
-// are: three instructions for four codes instead of five. For products whose
-// other operand is the same for all codes, so that 128 times its sum can be taken off once; the
-// sums then reach twice what they did, one bit of float32.
-__device__ __forceinline__ h8_t small8(uint32_t a, uint32_t b) {
-  a ^= 0x80808080u;
-  b ^= 0x80808080u;
-  return __builtin_bit_cast(h8_t, u4_t{__builtin_amdgcn_perm(0u, a, 0x0C010C00u), __builtin_amdgcn_perm(0u, a, 0x0C030C02u),
-                                       __builtin_amdgcn_perm(0u, b, 0x0C010C00u), __builtin_amdgcn_perm(0u, b, 0x0C030C02u)});
-}
-
 // Over the four lanes that differ in bits 4 and 5 of the lane.
 __device__ __forceinline__ float rows_max(float x) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from dance_amd import kv
-from test_kv import BF16, Model, check_attention, dev, fake, make, numbers, offsets_of
+from test_kv import BF16, F16, Model, check_attention, dev, fake, make, numbers, offsets_of
 
 # tokens over which a block repeats, sequences, rows of each, block tokens and dim: what joins the sums
 LONG = [
@@ -99,3 +99,20 @@ def test_batches_too_large_for_a_launch_are_refused(capfd):
     c, b, r = fake(seqs=1, tokens=1 << 30, max_tokens=1 << 30, table_width=1)
     assert kv._bind().dance_kv_attention(c, b, r, 1.0, 1 << 20, None, 1 << 20, 1 << 60, None) == -1
     assert "too large for one launch" in capfd.readouterr().err
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_logits_of_small_codes(dim, dt):
+    """Blocks whose scale an outlier set: their other codes are small, and a logit is no less exact for it."""
+    rng = np.random.default_rng(22)
+    lens = [1, 2, 17, 64, 700]
+    cache, table = make(rng, 2, dim, 32, lens)
+    cache.k.copy_(torch.from_numpy(np.rint(rng.normal(size=cache.k.shape)).astype(np.int8)))
+    cache.scale[..., 0] = 0.5
+    q = torch.from_numpy(rng.normal(size=(5, 6, dim)) + 2).to(dt).cuda()
+    got, lse = kv.attention(cache, q, dev(table), dev(np.int32(lens)), return_lse=True)
+    check_attention(Model(cache), got, lse, q, table, lens, offsets_of([1] * 5), dim ** -0.5)
+    lists = np.tile(np.arange(22, dtype=np.int32), (5, 2, 1))
+    got, lse = kv.sparse_attention(cache, q, dev(lists), dev(table), dev(np.int32(lens)), return_lse=True)
+    check_attention(Model(cache), got, lse, q, table, lens, offsets_of([1] * 5), dim ** -0.5, lists)
