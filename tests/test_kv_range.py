@@ -14,9 +14,11 @@ LONG = [
     (40000, 1, 1, 128, 64),     # k_step, many splits: k_join
     (70000, 128, 1, 128, 64),   # k_step, few splits: k_join_few
     (140000, 1100, 1, 64, 64),  # k_step, one split
-    (40000, 1, 200, 128, 128),  # k_chunk, many splits
+    (40000, 1, 200, 128, 128),  # k_step, many splits of many row tiles
     (140000, 256, 100, 64, 64),  # k_chunk, one split
     (40000, 1, 300, 128, 256),  # k_chunk, one wave a SIMD
+    (40000, 1, 500, 128, 128),  # k_chunk, many splits
+    (140000, 256, 130, 64, 64),  # k_chunk, one split, two row tiles
 ]
 
 
