@@ -82,3 +82,13 @@ def test_prune_kernels_hardly_spill(notes):
     sizes = {k: v for k, v in kernels(notes, "private_segment_fixed_size").items() if "k_prune" in k}
     assert len(sizes) > 20
     assert {k: v for k, v in sizes.items() if v > 40} == {}
+
+
+def test_cache_operators_fit_registers_and_lds(notes):
+    """Attention's tiles and append's rows stay in registers; the selection, held to 128 of them by 16 waves
+    a workgroup, keeps at most ten values a lane in scratch. With its 96 KB of keys it fits a CU's LDS."""
+    scratch, lds = (kernels(notes, f) for f in ("private_segment_fixed_size", "group_segment_fixed_size"))
+    ours = [k for k in scratch if "dance2kv" in k]
+    assert len(ours) > 100
+    assert {k: scratch[k] for k in ours if scratch[k] > (40 if "k_select" in k or "k_score" in k else 0)} == {}
+    assert {k: lds[k] for k in ours if lds[k] + (98304 if "k_select" in k else 0) > 163840} == {}
