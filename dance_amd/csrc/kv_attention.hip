@@ -60,11 +60,12 @@ constexpr uint32_t kRowTile = 16;
 // KB) 16.0 and 13.8 + 3.9 us, 128 of 4096 x 128 (1 MB) 42.5 and 31.0 + 4.1 us.
 constexpr uint32_t kWideWaves = 8;
 constexpr uint64_t kWideUnits = 256, kWideBytes = 256 << 10;
-// k_chunk for sequences of more than 64 rows (of a kv head, on average) where that is expected to
-// be faster. k_step's time goes with its row tiles x (tokens that they see + 128), k_chunk's with the longest
+// k_chunk for sequences of more than 64 rows (of a kv head, on average; 256 at 192 dimensions, where a
+// workgroup of 128 rows that is not full costs more than it gains) where that is expected to be faster. k_step's time goes with its row tiles x (tokens that they see + 128), k_chunk's with the longest
 // chain of tiles in a workgroup, which splits keep from growing beyond some 12; both in tiles of 64 tokens, and
 // the ratio by measurement. Of 901 shapes (64 to 256 dimensions; 8, 12 and 2 kv heads; 1 to 32 sequences; 40 to 8192 rows; 128
-// to 32,768 tokens) calls take 1.2 % more on average than with the faster kernel, 29 % where 64 rows alone decide.
+// to 32,768 tokens) calls take 1.2 % more on average than with the faster kernel, 29 % where 64 rows alone decide; of
+// 139 ragged batches 3.7 %.
 // Measured, whole calls (bf16, 8 kv heads of 4; prompts without and rows behind earlier tokens), k_step and k_chunk:
 //   dim  sequences x rows / tokens   us              dim  sequences x rows / tokens   us
 //   128  1 x 1024 / 256       9 and 13               64   1 x 256 / 8192      26 and 29
@@ -73,14 +74,15 @@ constexpr uint64_t kWideUnits = 256, kWideBytes = 256 << 10;
 //   128  8 x 2048 / 512     118 and 54               64   32 x 256 / 8192    382 and 244
 //   128  1 x 96 / 8192       24 and 31               192  1 x 2048 / 512      24 and 31
 //   128  1 x 256 / 8192      40 and 35               192  8 x 1024 / 256      64 and 41
-//   128  8 x 96 / 600        15 and 25               256  1 x 96 / 8192       43 and 48
-//   128  32 x 256 / 8192    726 and 383              256  32 x 72 / 8192     612 and 476
+//   128  8 x 96 / 600        15 and 25               192  8 x 192 / 8192     178 and 204
+//   128  32 x 256 / 8192    726 and 383              192  32 x 256 / 8192    881 and 765
+//   256  1 x 96 / 8192       43 and 48               256  32 x 72 / 8192     612 and 476
 // The average, because k_step's grid goes by the rows: 63 single tokens beside a prompt's 512, over 8192 each,
 // 128 dimensions (36 rows) take 368 and 528 us, beside 2048 (132 rows) 822 and 580. The lengths are not known here
 // but for the longest: prompts as ragged as 3 to 1270 tokens (12 heads of 96) take 24 and 34 us.
 bool chunk_pays(uint32_t dim, uint64_t heads, uint64_t group, uint64_t tokens, uint64_t seqs, uint64_t longest) {
   const uint64_t rows = group * tokens / seqs, own = tokens / seqs < longest ? tokens / seqs : longest;
-  if (rows <= 64) return false;
+  if (rows <= (dim == 192 ? 255 : 64)) return false;
   const uint64_t row_tiles = heads / group * seqs * ((rows + kRowTile - 1) / kRowTile), seen = longest - own / 2;
   const uint64_t chain = (longest + 63) / 64 < 12 ? (longest + 63) / 64 : 12;
   return row_tiles * (128 + seen) / 64 >= (dim <= 192 ? 1280 : 800) * chain;

@@ -154,6 +154,8 @@ RULE = [
     (8, 4, 128, 128, [128] * 8, True),           # short prompts: many, and one
     (8, 4, 128, 256, [256], False),
     (8, 4, 64, 8192, [8], False),
+    (8, 4, 192, 8192, [48] * 8, False),
+    (8, 4, 192, 8192, [64] * 8, True),
     (8, 4, 64, 8192, [32] * 32, True),
 ]
 
@@ -187,7 +189,7 @@ CHUNKS = [
     (16, 1, 64, 16, BF16, [140 + 7 * i for i in range(9)], [140] * 9, 4, 900),
     (8, 2, 96, 32, BF16, [90 + 3 * i for i in range(16)], [90] * 16, 4, 400),
     (16, 1, 128, 128, F16, [600, 131, 130, 0, 1000, 128, 77, 500], [130, 131, 130, 1, 129, 128, 77, 500], 4, 0),
-    (16, 1, 192, 64, BF16, [300] * 4 + [513, 150, 150, 150], [150] * 8, 4, 20),
+    (16, 1, 192, 64, BF16, [300] * 4 + [513, 270, 270, 261], [260] * 8, 4, 20),
     (16, 1, 256, 32, BF16, [300] * 4 + [513, 150, 150, 150], [150] * 8, 4, 0),
     (4, 2, 128, 16, BF16, [(37 * i) % 301 for i in range(70)], [(37 * i) % 301 for i in range(70)], 4, 0),  # 70 sequences
     (32, 1, 64, 64, F16, [520 + 9 * i for i in range(8)], [520] * 8, 8, 0),
