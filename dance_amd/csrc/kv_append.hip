@@ -6,12 +6,14 @@
 // doubles its scale, so that re-rounding its old codes moves a value by less
 // than one step of the final scale however often it grows; and any order or
 // precision of the arithmetic gives the same codes.
+// What a block that held tokens before holds behind its last one is not kept: of the 16 values that are
+// written together those are zeros.
 //
 // One workgroup per (sequence, touched block, head) and for keys and values
 // apart: the scale is a maximum over exactly that, so one launch finds it and
 // writes the codes, and the second read of the rows comes from the cache.
-// Measured: 64 sequences of one token, 8 heads of 128, 9.0 us, a chain of dependent loads
-// (length, table, rows, scale); 7,150 tokens of 16 prompts 20.5 us, 2.1 TB/s of
+// Measured: 64 sequences of one token, 8 heads of 128, 9.2 us, a chain of dependent loads
+// (length, table, rows, scale); 7,105 tokens of 16 prompts 21 us, 2.1 TB/s of
 // compulsory bytes, the same chain in eight workgroups a CU.
 
 #include <cmath>

@@ -30,11 +30,11 @@
 // l where its weight is more than 2^-41 times their scale of theirs (p is then a normal number).
 //
 // Bound by the codes' bytes: a step reads each once and does 4 operations on it per row. Measured (8 kv
-// heads of 4, 128 dimensions): 64 sequences of 500 to 12,000 tokens, 497 MB, 104 us (4.8 TB/s, a large copy's rate);
-// 2 of 400,000 to 600,000, 461 MB, 85 us (5.4 TB/s) and 11 of join; 16 rows over 64 listed blocks
-// of 64 tokens each, 135 MB, 27 us (5.0 TB/s). One sequence of 700 tokens takes 9.6 us, a chain of dependent loads.
-// Lists of 1026 rows over the same 145 MB are bound by instructions (64 % of the cycles) and by
-// what the L2s miss of them (1.4 GB): 301 us.
+// heads of 4, 128 dimensions): 64 sequences of 500 to 12,000 tokens, 497 MB, 105 us (4.7 TB/s; a stream that only
+// reads reaches 6.5, a large copy 4.8); 2 of 400,000 to 600,000, 461 MB, 85 us (5.4 TB/s) and 11 of join; 16 rows over
+// 64 listed blocks of 64 tokens each, 135 MB, 28 us (4.7 TB/s). One sequence of 700 tokens takes 9.8 us, a chain of
+// dependent loads. Lists of 1026 rows over the same 145 MB are bound by instructions (64 % of the cycles) and by
+// what the L2s miss of them (1.4 GB): 312 us.
 
 #include <cfloat>
 #include <cmath>
@@ -55,9 +55,9 @@ constexpr uint32_t kRowTile = 16;
 // Waves of a workgroup that takes all of a row tile's tokens. It needs no join (and
 // its launch), but a CU reads 75 GB/s at most: up to one workgroup per CU and
 // kWideBytes of codes for each, more where many keep the chip busy anyway. Measured
-// with it and with splits, of 128 dimensions (whole calls): 8 units of 1024 tokens
-// 11.6 and 13.5 us, of 2048 16.7 and 14.1; kernels alone: 216 units of 3500 x 64 (448
-// KB) 16.0 and 13.8 + 3.9 us, 128 of 4096 x 128 (1 MB) 42.5 and 31.0 + 4.1 us.
+// with it and with splits, whole calls: of 128 dimensions 8 units of 1024 tokens 11.2 and 11.1 us, of 2048 16.3 and
+// 14.2, 256 of 2048 (512 KB) 23.6 and 27.0, 128 of 4096 (1 MB) 29.0 and 27.2; of 64 dimensions 72 units of 3000 (384 KB)
+// 14.8 and 13.0, 128 of 3000 15.5 and 16.5, 216 of 3500 (448 KB) 19.7 and 24.1.
 constexpr uint32_t kWideWaves = 8;
 constexpr uint64_t kWideUnits = 256, kWideBytes = 256 << 10;
 // k_chunk for sequences of more than 64 rows (of a kv head, on average; 256 at 192 dimensions, where a
@@ -88,9 +88,9 @@ bool chunk_pays(uint32_t dim, uint64_t heads, uint64_t group, uint64_t tokens, u
   return row_tiles * (128 + seen) / 64 >= (dim <= 192 ? 1280 : 800) * chain;
 }
 // Its workgroups have eight waves where that gives each CU two of them, else four:
-// 627 and 653 us for two chunks of 2048 tokens over 6000 to 10000, 42 and 36 us for
+// 521 and 557 us for two chunks of 2048 tokens over 6000 to 10000, 41 and 34 us for
 // 1024 over 1024. Below one workgroup per CU the tokens are split, up to kChunkUnits workgroups
-// of at least kChunkSplitTiles tiles (64 tokens over 8192: 32 us at 8 tiles, 41 at 16).
+// of at least kChunkSplitTiles tiles (64 tokens over 8192: 38 us at 8 tiles, 42 at 16).
 constexpr uint64_t kChunkSplitTiles = 8;
 constexpr uint64_t kChunkUnits = 512;
 constexpr int kChunkWide = 8, kChunkSmall = 4;
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 #include "kv_chunk.h"
 
 // Joins a row's few splits. Every lane has four dimensions and reads all
-// splits' references itself, so that nothing is exchanged (7 ragged prompts, 12 heads of 96, 3
+// splits' references itself, so that nothing is exchanged (7 ragged prompts, 12 heads of 96, 2
 // splits: 6.4 us, bound by the splits' bytes; a wave a row that exchanged them 9.1).
 template <int D, bool BF>
 __global__ __launch_bounds__(kJoinThreads) void k_join_few(const float* __restrict__ part, uint32_t splits, uint64_t rows,

@@ -12,8 +12,8 @@
 // operand wants: within 16 tokens 0-3, 8-11, 4-7, 12-15, a swap of words.
 //
 // Bound by the softmax's and the conversion's vector instructions and the matrix units in turn: two chunks of
-// 2048 tokens over 6,000 to 10,000, 8 kv heads of 4, 128 dimensions (491 GFLOP), 533 us, 922 TFLOP/s; a
-// large f16 product reaches 1136. Vector instructions are 51 %, matrix instructions 34 % of the time.
+// 2048 tokens over 6,000 to 10,000, 8 kv heads of 4, 128 dimensions (491 GFLOP), 528 us, 930 TFLOP/s; a
+// large f16 product reaches 1370. Vector instructions are 50 %, matrix instructions 38 % of the time.
 #pragma once
 
 constexpr int chunk_occ(int d) { return d <= 128 ? 2 : 1; }  // waves per SIMD, by registers

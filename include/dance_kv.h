@@ -1,9 +1,9 @@
 /* A key-value cache in 8-bit codes and the operators that write it and read
  * it: append, attention over all of a sequence, the selection of the blocks
  * worth reading by a bound on their keys' products with the query, and
- * attention over selected blocks. No counterpart in the reference: these carry
- * the library's code rows, bounds and top-k searches to the keys and values of
- * a language model's cache.
+ * attention over selected blocks. No counterpart in the reference: beside the
+ * library's searches over vectors in 8-bit codes, the same idea for the keys and
+ * values of a language model's cache, with layouts and kernels of their own.
  *
  * All pointers are device pointers. A call checks its arguments on the host,
  * launches its kernels on `stream` and returns; it allocates nothing, waits
@@ -80,7 +80,8 @@ typedef struct DanceKvRows {
  * none of the sequence's tokens before), its old codes c become rint(c * s / s')
  * and the new ones rint(x / s'), halves to even. Not finite: infinities take
  * the code +-127, NaN the code 0, and neither counts for a. The bounds follow.
- * A block that the call opens holds zeros behind its last token. Two
+ * A block that the call opens holds zeros behind its last token, others hold
+ * anything there (tokens that a shorter length gave up are not kept). Two
  * sequences, or two places of one, must not share a block that is written. */
 int dance_kv_append(const DanceKvCache *cache, const DanceKvBatch *batch, const DanceKvRows *keys,
                     const DanceKvRows *values, void *stream);
