@@ -1,4 +1,5 @@
-// dance_kv_attention and dance_kv_sparse_attention (include/dance_kv.h).
+// dance_kv_attention and dance_kv_sparse_attention (include/dance_kv.h), dance_kv_cross_attention
+// (include/dance_kv_parts.h).
 //
 // For a tile of 64 tokens (32 at 256 dimensions) and 16 query rows a wave forms S' = K Q' (tokens x
 // rows) and then O' += V' P' (dims x rows) with 16x16x32 f16 MFMAs. Codes are
@@ -40,6 +41,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "../../include/dance_kv_parts.h"
 #include "kv_common.h"
 
 namespace dance {
@@ -80,8 +82,8 @@ constexpr uint64_t kWideUnits = 256, kWideBytes = 256 << 10;
 // The average, because k_step's grid goes by the rows: 63 single tokens beside a prompt's 512, over 8192 each,
 // 128 dimensions (36 rows) take 368 and 528 us, beside 2048 (132 rows) 822 and 580. The lengths are not known here
 // but for the longest: prompts as ragged as 3 to 1270 tokens (12 heads of 96) take 24 and 34 us.
-bool chunk_pays(uint32_t dim, uint64_t heads, uint64_t group, uint64_t tokens, uint64_t seqs, uint64_t longest) {
-  const uint64_t rows = group * tokens / seqs, own = tokens / seqs < longest ? tokens / seqs : longest;
+bool chunk_pays(uint32_t dim, uint64_t heads, uint64_t group, uint64_t tokens, uint64_t seqs, uint64_t longest, bool full) {
+  const uint64_t rows = group * tokens / seqs, own = full ? 0 : tokens / seqs < longest ? tokens / seqs : longest;
   if (rows <= (dim == 192 ? 255 : 64)) return false;
   const uint64_t row_tiles = heads / group * seqs * ((rows + kRowTile - 1) / kRowTile), seen = longest - own / 2;
   const uint64_t chain = (longest + 63) / 64 < 12 ? (longest + 63) / 64 : 12;
@@ -114,6 +116,7 @@ struct StepArgs {
   uint16_t* __restrict__ out;
   float* __restrict__ lse;
   float* __restrict__ part;  // splits > 1: [row][split][D] sums, then [row][split][2] (R, l)
+  bool full;                 // rows see all tokens, whatever their own place
 };
 
 // A sum of many tiles with what its additions rounded off: without it the logarithm of 140,000
@@ -207,7 +210,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   const uint32_t r = r_first + min(n, rows - 1u);
   const uint32_t tok = r / a.group, head = h * a.group + r % a.group;
   // last position that this lane's row sees, and that any row of the tile does
-  const int64_t p_row = min(s.first + tok, s.len - 1), p_top = min(s.first + (r_first + rows - 1) / a.group, s.len - 1);
+  const int64_t p_all = s.len - 1, p_row = a.full ? p_all : min(s.first + tok, p_all);
+  const int64_t p_top = a.full ? p_all : min(s.first + (r_first + rows - 1) / a.group, p_all);
   const int32_t pos = n < rows && p_row >= 0 ? (int32_t)p_row : -1, top = p_top >= 0 ? (int32_t)p_top : -1;
   const int32_t seen = (int32_t)((uint32_t)(top + 1 + (int32_t)bs - 1) >> bsh);  // blocks
   const int32_t* const list = LIST ? a.lists + ((size_t)id * a.c.kvh + h) * a.count : nullptr;
@@ -567,12 +571,15 @@ struct Plan {
   int waves;  // of a workgroup of k_chunk
   size_t work;
 };
-Plan plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, bool list, uint32_t count) {
+enum Kind { kCausal, kFull, kList };
+Plan plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, Kind kind, uint32_t count) {
+  const bool list = kind == kList;
   Plan p{};
   if (b->tokens == 0) return p;
   const uint64_t group = heads / c->kv_heads;
   const uint64_t rows = list ? group : group * b->max_tokens;
-  p.chunk = !list && chunk_pays(c->dim, heads, group, b->tokens, b->seqs, (uint64_t)most_blocks(c, b) * c->block_tokens);
+  p.chunk = !list && chunk_pays(c->dim, heads, group, b->tokens, b->seqs, (uint64_t)most_blocks(c, b) * c->block_tokens,
+                               kind == kFull);
   // by the rows that there are: sequences may have fewer than max_tokens
   const uint64_t big = 32 * kChunkWide;
   p.waves = c->dim <= 128 && (group * b->tokens + big - 1) / big * c->kv_heads >= kChunkUnits ? kChunkWide : kChunkSmall;
@@ -606,8 +613,9 @@ bool count_fits(const DanceKvCache* c, uint32_t count) {
 }
 
 int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, const DanceKvRows* q,
-        const int32_t* lists, bool list, uint32_t count, float scale, void* out, float* lse, void* work,
+        const int32_t* lists, Kind kind, uint32_t count, float scale, void* out, float* lse, void* work,
         size_t work_bytes, void* stream) {
+  const bool list = kind == kList;
   const char* why = check_common(cache, batch);
   if (!why) why = check_rows(cache, q, false);
   if (!why && (!out || !aligned(out, 16))) why = "out must be given, aligned to 16 bytes";
@@ -619,7 +627,7 @@ int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, c
     return -1;
   }
   if (batch->tokens == 0) return 0;
-  const Plan p = plan(cache, batch, q->heads, list, count);
+  const Plan p = plan(cache, batch, q->heads, kind, count);
   if (p.work && (!work || work_bytes < p.work || !aligned(work, 16))) {
     std::fprintf(stderr, "[%s] work must hold %zu bytes, aligned to 16\n", who, p.work);
     return -1;
@@ -636,7 +644,7 @@ int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, c
   const hipStream_t st = static_cast<hipStream_t>(stream);
   StepArgs a{cache_args(cache), batch_args(batch), rows_args(q), lists, count, scale * kLog2e,
              q->heads / cache->kv_heads, p.tiles, p.slots, p.splits, p.per, static_cast<uint16_t*>(out), lse,
-             static_cast<float*>(work)};
+             static_cast<float*>(work), kind == kFull};
   const bool vec = rows_vector(q);
   with_kind(cache->dim, q->dtype, [&](auto d, auto bf) {
     constexpr int D = decltype(d)::value;
@@ -684,25 +692,37 @@ extern "C" {
 
 int dance_kv_attention(const DanceKvCache* cache, const DanceKvBatch* batch, const DanceKvRows* queries, float scale,
                        void* out, float* lse, void* work, size_t work_bytes, void* stream) {
-  return run("dance_kv_attention", cache, batch, queries, nullptr, false, 0, scale, out, lse, work, work_bytes, stream);
+  return run("dance_kv_attention", cache, batch, queries, nullptr, kCausal, 0, scale, out, lse, work, work_bytes,
+             stream);
 }
 
 size_t dance_kv_attention_work(const DanceKvCache* cache, const DanceKvBatch* batch, uint32_t heads) {
   if (check_shapes(cache, batch) || heads == 0 || heads % cache->kv_heads) return 0;
-  return plan(cache, batch, heads, false, 0).work;
+  return plan(cache, batch, heads, kCausal, 0).work;
+}
+
+int dance_kv_cross_attention(const DanceKvCache* cache, const DanceKvBatch* batch, const DanceKvRows* queries, float scale,
+                             void* out, float* lse, void* work, size_t work_bytes, void* stream) {
+  return run("dance_kv_cross_attention", cache, batch, queries, nullptr, kFull, 0, scale, out, lse, work, work_bytes,
+             stream);
+}
+
+size_t dance_kv_cross_attention_work(const DanceKvCache* cache, const DanceKvBatch* batch, uint32_t heads) {
+  if (check_shapes(cache, batch) || heads == 0 || heads % cache->kv_heads) return 0;
+  return plan(cache, batch, heads, kFull, 0).work;
 }
 
 int dance_kv_sparse_attention(const DanceKvCache* cache, const DanceKvBatch* batch, const DanceKvRows* queries,
                               const int32_t* lists, uint32_t count, float scale, void* out, float* lse, void* work,
                               size_t work_bytes, void* stream) {
-  return run("dance_kv_sparse_attention", cache, batch, queries, lists, true, count, scale, out, lse, work, work_bytes,
+  return run("dance_kv_sparse_attention", cache, batch, queries, lists, kList, count, scale, out, lse, work, work_bytes,
              stream);
 }
 
 size_t dance_kv_sparse_attention_work(const DanceKvCache* cache, const DanceKvBatch* batch, uint32_t heads,
                                       uint32_t count) {
   if (check_shapes(cache, batch) || heads == 0 || heads % cache->kv_heads || !count_fits(cache, count)) return 0;
-  return plan(cache, batch, heads, true, count).work;
+  return plan(cache, batch, heads, kList, count).work;
 }
 
 }  // extern "C"

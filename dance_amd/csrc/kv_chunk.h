@@ -61,7 +61,7 @@ __global__ __launch_bounds__(64 * W)
   const uint32_t r_first = (tiles - 1u - at.tile) * kRows;
   const uint32_t rows = min(kRows, r_end - r_first);
   auto pos_of = [&](uint32_t r) {
-    const int64_t p = min(s.first + r / a.group, s.len - 1);
+    const int64_t p = a.full ? s.len - 1 : min(s.first + r / a.group, s.len - 1);
     return p >= 0 ? (int32_t)p : -1;
   };
   auto row_of = [&](uint32_t rr) {

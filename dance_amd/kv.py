@@ -1,11 +1,24 @@
 """A key-value cache in 8-bit codes and attention over it, or over the blocks
-that a bound on their keys selects: Python front-end of include/dance_kv.h.
+that a bound on their keys selects: Python front-end of include/dance_kv.h,
+dance_kv_parts.h and dance_kv_pages.h.
 
     cache = KVCache.empty(blocks, kv_heads, dim, block_tokens=64)
     append(cache, k, v, table, lengths)                      # a step's or a prompt's tokens
     o = attention(cache, q, table, lengths)                  # over all tokens
     chosen = select(cache, q, table, lengths, 64, sink=1, recent=2)
     o = sparse_attention(cache, q, chosen, table, lengths)   # over 64 blocks a query
+    o = cross_attention(cache, q, table, lengths)            # rows that see all of another sequence
+    o = join([o, other], [lse, other_lse])                   # attentions over parts of a context
+
+and the owners of its blocks, for sequences that fork, grow and shrink:
+
+    pages = Pages.empty(blocks, block_tokens=64)
+    table, lengths = fork(pages, table, lengths, parents)    # row i goes on from row parents[i]
+    now, src, dst = reserve(pages, table, lengths, lengths + 1)
+    copy(caches, src, dst)                                   # shared blocks that are about to be written, in all layers
+    append(cache, k, v, table, now)
+    release(pages, table, lengths, keep=lengths - 2)         # the last two tokens go
+    compact(cache, keep, counts, table, lengths, new_table)  # chosen tokens move to blocks of their own
 
 Arguments that all calls share:
     table    [sequences, blocks] int32: the cache block of each part of a
@@ -54,10 +67,21 @@ class DanceKvRows(C.Structure):
                 ("dtype", C.c_int)]
 
 
+class DanceKvPart(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64), ("lse", C.c_void_p),
+                ("rows", C.c_void_p), ("tokens", C.c_uint64)]
+
+
+class DanceKvPages(C.Structure):
+    _fields_ = [("refs", C.c_void_p), ("blocks", C.c_uint32), ("block_tokens", C.c_uint32)]
+
+
 # The same structs as bytes, which a call takes as it takes a pointer: a small
 # attention is 8 us of host time, and the three ctypes objects would be another 1.5.
 _CACHE, _BATCH, _ROWS = struct.Struct("@PPPPIIII"), struct.Struct("@PPPIIIIQ"), struct.Struct("@PqqIi")
-assert [_CACHE.size, _BATCH.size, _ROWS.size] == [C.sizeof(t) for t in (DanceKvCache, DanceKvBatch, DanceKvRows)]
+_PART, _PAGES = struct.Struct("@PqqPPQ"), struct.Struct("@PII")
+assert [_CACHE.size, _BATCH.size, _ROWS.size, _PART.size, _PAGES.size] == [
+    C.sizeof(t) for t in (DanceKvCache, DanceKvBatch, DanceKvRows, DanceKvPart, DanceKvPages)]
 
 # torch's handle of the current stream, without the Stream object around it where torch has that
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -75,6 +99,7 @@ def _bind():
         L = _lib()
         vp, u32, f32, sz = C.c_void_p, C.c_uint32, C.c_float, C.c_size_t
         cache, batch, rows = C.POINTER(DanceKvCache), C.POINTER(DanceKvBatch), C.POINTER(DanceKvRows)
+        part, pages = C.POINTER(DanceKvPart), C.POINTER(DanceKvPages)
         for name, args, res in (
                 ("append", [cache, batch, rows, rows, vp], C.c_int),
                 ("attention", [cache, batch, rows, f32, vp, vp, vp, sz, vp], C.c_int),
@@ -82,10 +107,19 @@ def _bind():
                 ("select", [cache, batch, rows, u32, u32, u32, vp, vp, sz, vp], C.c_int),
                 ("select_work", [cache, batch, u32, u32], sz),
                 ("sparse_attention", [cache, batch, rows, vp, u32, f32, vp, vp, vp, sz, vp], C.c_int),
-                ("sparse_attention_work", [cache, batch, u32, u32], sz)):
+                ("sparse_attention_work", [cache, batch, u32, u32], sz),
+                ("cross_attention", [cache, batch, rows, f32, vp, vp, vp, sz, vp], C.c_int),
+                ("cross_attention_work", [cache, batch, u32], sz),
+                ("join", [part, u32, u32, u32, u32, C.c_int, vp, vp, vp], C.c_int),
+                ("fork", [pages, vp, vp, u32, u32, vp, u32, vp, vp, vp], C.c_int),
+                ("reserve", [pages, vp, vp, u32, u32, vp, vp, vp, vp, vp, sz, vp], C.c_int),
+                ("reserve_work", [pages, u32, u32], sz),
+                ("release", [pages, vp, vp, u32, u32, vp, vp, vp], C.c_int),
+                ("copy", [cache, cache, u32, vp, vp, u32, vp], C.c_int),
+                ("compact", [cache, cache, vp, vp, u32, u32, vp, u32, u32, vp, vp, u32, vp], C.c_int)):
             fn = getattr(L, "dance_kv_" + name)
             fn.argtypes, fn.restype = args, res
-            as_bytes = [C.c_char_p if t in (cache, batch, rows) else t for t in args]
+            as_bytes = [C.c_char_p if t in (cache, batch, rows, part, pages) else t for t in args]
             _fast[name] = C.CFUNCTYPE(res, *as_bytes)(("dance_kv_" + name, L))
         _bound = L
     return _bound
@@ -133,6 +167,29 @@ class KVCache:
         return cls(make((blocks, kv_heads, block_tokens, dim), torch.int8),
                    make((blocks, kv_heads, dim, block_tokens), torch.int8), make((blocks, kv_heads, 2), torch.float32),
                    make((blocks, kv_heads, 2, dim), torch.int8))
+
+
+class Pages:
+    """The owners of a pool's blocks: refs [blocks] int32 counts the table entries
+    that name a block (a caller may count others there to keep it); 0 is free."""
+
+    def __init__(self, refs, block_tokens=64):
+        if refs.dtype != torch.int32 or refs.ndim != 1:
+            raise TypeError("refs must be a 1-dimensional int32 tensor")
+        if refs.shape[0] < 1 or not refs.is_contiguous():
+            raise ValueError("refs must be contiguous and not empty")
+        if block_tokens not in BLOCK_TOKENS:
+            raise ValueError(f"block_tokens must be one of {BLOCK_TOKENS}")
+        if refs.device.type != "cuda":
+            raise ValueError("refs must be in GPU memory")
+        self.refs, self.blocks, self.block_tokens, self.device = refs, refs.shape[0], block_tokens, refs.device
+        self._bytes = _PAGES.pack(refs.data_ptr(), self.blocks, block_tokens)
+        _bind()
+
+    @classmethod
+    def empty(cls, blocks, block_tokens=64, device="cuda"):
+        """A pool whose blocks are all free."""
+        return cls(torch.zeros(blocks, dtype=torch.int32, device=device), block_tokens)
 
 
 def _ints(name, t, shape, device):
@@ -189,15 +246,18 @@ def _batch(cache, tokens, table, lengths, offsets, max_tokens, max_length):
                        max_length or 0)
 
 
-def _call(name, cache, *args):
-    index = cache.device.index
+def _launch(name, index, *args):
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
-            rc = _fast[name](cache._bytes, *args, _stream(index))
+            rc = _fast[name](*args, _stream(index))
     else:
-        rc = _fast[name](cache._bytes, *args, _stream(index))
+        rc = _fast[name](*args, _stream(index))
     if rc != 0:
         raise RuntimeError(f"dance_kv_{name} failed with return code {rc}")
+
+
+def _call(name, cache, *args):
+    _launch(name, cache.device.index, cache._bytes, *args)
 
 
 def _work(cache, size):
@@ -283,3 +343,171 @@ def sparse_attention(cache, q, chosen, table, lengths, offsets=None, *, scale=No
         _call("sparse_attention", cache, b, r, chosen.data_ptr(), count, cache.dim ** -0.5 if scale is None else scale,
               out.data_ptr(), _ptr(lse), _ptr(work), size)
     return (out, lse) if return_lse else out
+
+
+def cross_attention(cache, q, table, lengths, offsets=None, *, scale=None, max_tokens=None, max_length=None, out=None,
+                    return_lse=False):
+    """attention whose rows see all tokens of their sequence, whatever their own place:
+    an encoder's states, or a prefix that the rows of many sequences share. lengths
+    has no rows of this call in it."""
+    r, tokens, heads = _rows(cache, "q", q)
+    b = _batch(cache, tokens, table, lengths, offsets, max_tokens, max_length)
+    out = _out(out, q)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=cache.device) if return_lse else None
+    if tokens:
+        size = _fast["cross_attention_work"](cache._bytes, b, heads)
+        work = _work(cache, size)
+        _call("cross_attention", cache, b, r, cache.dim ** -0.5 if scale is None else scale, out.data_ptr(), _ptr(lse),
+              _ptr(work), size)
+    return (out, lse) if return_lse else out
+
+
+def join(parts, lses, rows=None, *, out=None, return_lse=False):
+    """The attention over a context from those over 1 to 8 parts of it: parts [tokens,
+    heads, dim] of one type, and the logarithms of their sums, [tokens, heads]
+    float32, as return_lse gives them. Rows whose logarithm is -inf count for
+    nothing. rows: for each part None, or [joined tokens] int32 with the part's row
+    for each joined one, and anything outside the part where it has none."""
+    count = len(parts)
+    if not 1 <= count <= 8 or len(lses) != count or (rows is not None and len(rows) != count):
+        raise ValueError("1 to 8 parts, and as many lses and rows")
+    first = parts[0]
+    if first.ndim != 3:
+        raise ValueError("parts must be [tokens, heads, dim]")
+    _, heads, dim = first.shape
+    dtype, device = first.dtype, first.device
+    if dtype not in DTYPES:
+        raise TypeError("parts must be float16 or bfloat16")
+    if device.type != "cuda":
+        raise ValueError("parts must be in GPU memory")
+    if heads < 1 or dim < 1:
+        raise ValueError("parts must have heads and dimensions")
+    tokens, args = None, []
+    for i, (x, lse) in enumerate(zip(parts, lses)):
+        at = rows[i] if rows is not None else None
+        if x.ndim != 3 or x.shape[1:] != first.shape[1:]:
+            raise ValueError("parts must have one number of heads and dimensions")
+        if x.dtype != dtype:
+            raise TypeError("parts must have one type")
+        if x.device != device or x.stride(2) != 1 and dim > 1:
+            raise ValueError("parts must be on one device, with adjacent dimensions")
+        if lse.dtype != torch.float32:
+            raise TypeError("lses must be float32")
+        if lse.shape != x.shape[:2] or lse.device != device or not lse.is_contiguous():
+            raise ValueError("lses must be contiguous, [tokens, heads], on the parts' device")
+        if at is not None:
+            _ints("rows", at, at.shape[:1], device)
+        n = x.shape[0] if at is None else at.shape[0]
+        if tokens is not None and n != tokens:
+            raise ValueError("parts, or their rows, must have one number of tokens")
+        tokens = n
+        args.append(_PART.pack(x.data_ptr(), x.stride(0), x.stride(1), lse.data_ptr(), _ptr(at) or 0, x.shape[0]))
+    shape = (tokens, heads, dim)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=device)
+    elif out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {dtype} tensor {shape} on the parts' device")
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
+    _bind()
+    if tokens:
+        _launch("join", device.index, b"".join(args), count, tokens, heads, dim, DTYPES[dtype], out.data_ptr(), _ptr(lse))
+    return (out, lse) if return_lse else out
+
+
+def _table(pages, table, lengths):
+    shape = table.shape
+    if len(shape) != 2 or 0 in shape:
+        raise ValueError("table must be [sequences, blocks]")
+    _ints("table", table, shape, pages.device)
+    _ints("lengths", lengths, shape[:1], pages.device)
+    return shape
+
+
+def fork(pages, table, lengths, parents):
+    """A new table and its lengths: row i is row parents[i] ([new sequences] int32) of
+    the old ones, which end; a parent outside the table gives an empty row. Beams
+    that go on from others, samples of one prompt, slots that end."""
+    seqs, width = _table(pages, table, lengths)
+    new = parents.shape[0] if parents.ndim == 1 else 0
+    if new == 0:
+        raise ValueError("parents must be [new sequences]")
+    _ints("parents", parents, (new,), pages.device)
+    new_table = torch.empty((new, width), dtype=torch.int32, device=pages.device)
+    new_lengths = torch.empty(new, dtype=torch.int32, device=pages.device)
+    _call("fork", pages, table.data_ptr(), lengths.data_ptr(), seqs, width, parents.data_ptr(), new, new_table.data_ptr(),
+          new_lengths.data_ptr())
+    return new_table, new_lengths
+
+
+def reserve(pages, table, lengths, upto):
+    """Room for the tokens up to upto [sequences] int32, in blocks that each sequence
+    alone owns; table and lengths change in place. Returns (now, src, dst), each [sequences]
+    int32: now is the lengths to append with, upto where there was room and 0 (nothing is
+    written) where there was not; copy has to take the blocks src to dst before anything
+    is written. Sequences and their places take the free blocks in ascending order."""
+    seqs, width = _table(pages, table, lengths)
+    _ints("upto", upto, (seqs,), pages.device)
+    now, src, dst = torch.empty((3, seqs), dtype=torch.int32, device=pages.device).unbind(0)
+    size = _fast["reserve_work"](pages._bytes, seqs, width)
+    work = _work(pages, size)
+    _call("reserve", pages, table.data_ptr(), lengths.data_ptr(), seqs, width, upto.data_ptr(), now.data_ptr(), src.data_ptr(),
+          dst.data_ptr(), _ptr(work), size)
+    return now, src, dst
+
+
+def release(pages, table, lengths, keep=None, start=None):
+    """Gives blocks back, in place: with keep [sequences] int32 those behind the first
+    keep tokens, and lengths follow; with start those of which all tokens stand before
+    it, whose places become holes."""
+    seqs, width = _table(pages, table, lengths)
+    for name, t in (("keep", keep), ("start", start)):
+        if t is not None:
+            _ints(name, t, (seqs,), pages.device)
+    _call("release", pages, table.data_ptr(), lengths.data_ptr(), seqs, width, _ptr(keep), _ptr(start))
+
+
+def _alike(a, b):
+    if (a.kv_heads, a.dim, a.block_tokens, a.device) != (b.kv_heads, b.dim, b.block_tokens, b.device):
+        raise ValueError("the caches must have one kv_heads, dim, block_tokens and device")
+
+
+def copy(caches, src, dst, into=None):
+    """Copies the blocks src to dst ([pairs] int32, pairs outside the caches are left out) of one cache or of
+    each of a list (a model's layers), to the caches `into` if given (another pool)."""
+    caches = [caches] if isinstance(caches, KVCache) else list(caches)
+    into = caches if into is None else [into] if isinstance(into, KVCache) else list(into)
+    if not caches or len(into) != len(caches):
+        raise ValueError("there must be caches, and as many to copy into")
+    for side in (caches, into):
+        for c in side:
+            _alike(caches[0], c)
+            if c.blocks != side[0].blocks:
+                raise ValueError("the caches must have one number of blocks")
+    pairs = src.shape[0] if src.ndim == 1 else 0
+    _ints("src", src, (pairs,), caches[0].device)
+    _ints("dst", dst, (pairs,), caches[0].device)
+    if pairs:
+        _launch("copy", caches[0].device.index, b"".join(c._bytes for c in caches), b"".join(c._bytes for c in into),
+                len(caches), src.data_ptr(), dst.data_ptr(), pairs)
+
+
+def compact(cache, keep, counts, table, lengths, into_table, into=None):
+    """Writes chosen tokens densely into other blocks: token i < counts[b] of head h is
+    the one at position keep[b, h, i] of sequence b (keep [sequences, kv_heads or 1,
+    n] int32), and goes to the blocks of into_table [sequences, blocks] int32, of the cache `into` if
+    given. Blocks get the scales that append would give them. No block may be read and written."""
+    into = cache if into is None else into
+    _alike(cache, into)
+    shape = table.shape
+    if len(shape) != 2 or 0 in shape or into_table.ndim != 2 or 0 in into_table.shape:
+        raise ValueError("tables must be [sequences, blocks]")
+    seqs, width = shape
+    if keep.ndim != 3 or keep.shape[1] not in (1, cache.kv_heads) or keep.shape[2] < 1:
+        raise ValueError(f"keep must be [sequences, {cache.kv_heads} or 1, n]")
+    _ints("table", table, shape, cache.device)
+    _ints("lengths", lengths, (seqs,), cache.device)
+    _ints("counts", counts, (seqs,), cache.device)
+    _ints("keep", keep, (seqs, *keep.shape[1:]), cache.device)
+    _ints("into_table", into_table, (seqs, into_table.shape[1]), cache.device)
+    _call("compact", cache, into._bytes, table.data_ptr(), lengths.data_ptr(), seqs, width, keep.data_ptr(), keep.shape[1],
+          keep.shape[2], counts.data_ptr(), into_table.data_ptr(), into_table.shape[1])

@@ -1,7 +1,8 @@
 /* A key-value cache in 8-bit codes and the operators that write it and read
  * it: append, attention over all of a sequence, the selection of the blocks
  * worth reading by a bound on their keys' products with the query, and
- * attention over selected blocks. No counterpart in the reference: beside the
+ * attention over selected blocks (attention over parts of a context: dance_kv_parts.h; the
+ * blocks' owners, copies and compaction: dance_kv_pages.h). No counterpart in the reference: beside the
  * library's searches over vectors in 8-bit codes, the same idea for the keys and
  * values of a language model's cache, with layouts and kernels of their own.
  *

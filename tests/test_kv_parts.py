@@ -1,0 +1,330 @@
+"""Attention over parts of a context (include/dance_kv_parts.h, dance_amd/kv.py): rows that see all of another
+sequence, and joined attentions, against their definitions in 64 bits on the CPU.
+
+Cross attention has attention's tolerance (test_kv.py). A joined row is sum w_i o_i / sum w_i with w_i =
+exp(l_i - m): each weight is off by at most e_i = 2^-21 + |l_i - m| 2^-23 of itself (the difference's rounding, the
+exponential's within 4 units, products and sums of eight parts with 2^-24 each), once above and once below, so the row by
+u |o| + 2 sum w_i e_i |o_i| / sum w_i + half the least number of its type, and its logarithm by 2^-23 |l| + 2 max
+w_i e_i + 2^-22."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from dance_amd import kv
+from test_kv import BF16, F16, IDS, LEAST, PROMPTS, ROUND, SHAPES, Model, check_attention, dev, fake, make, numbers, offsets_of
+
+
+def check_cross(model, got, lse, q, table, lens, off, scale):
+    """Every row as a sequence of its own, whose last token it is."""
+    seq = np.repeat(np.arange(len(lens)), np.diff(off))
+    check_attention(model, got, lse, q, table[seq], [min(lens[b], table.shape[1] * model.bs) for b in seq],
+                    np.arange(len(seq) + 1), scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", SHAPES, ids=IDS)
+@pytest.mark.parametrize("holes", [0, 2])
+def test_cross_attention(shape, holes):
+    heads, group, dim, bs, dt, lens, news = shape
+    rng = np.random.default_rng(31)
+    cache, table = make(rng, heads, dim, bs, lens, holes)
+    off = offsets_of(news or [1] * len(lens))
+    q = torch.from_numpy(rng.normal(size=(off[-1], heads * group, dim))).to(dt).cuda()
+    got, lse = kv.cross_attention(cache, q, dev(table), dev(np.int32(lens)), dev(off) if news else None, return_lse=True,
+                                  max_tokens=max(news) if news else None)
+    check_cross(Model(cache), got, lse, q, table, lens, off, dim ** -0.5)
+
+
+# more rows than tokens, fewer, sequences without any, and lengths that the prompts' kernel takes
+MANY = PROMPTS + [(2, 4, 128, 64, F16, [5, 0, 300], [90, 70, 40]), (1, 4, 64, 32, BF16, [1, 33], [130, 1]),
+                  (1, 1, 192, 64, BF16, [700], [400]), (2, 8, 96, 16, F16, [2000, 17], [33, 64])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", MANY, ids=[f"{s[0]}x{s[1]}-{s[2]}-{s[3]}-{i}" for i, s in enumerate(MANY)])
+@pytest.mark.parametrize("holes,scale", [(0, None), (3, 0.3), (0, -0.1), (0, 0.0)])
+def test_cross_attention_of_many_rows(shape, holes, scale):
+    heads, group, dim, bs, dt, lens, news = shape
+    rng = np.random.default_rng(32)
+    cache, table = make(rng, heads, dim, bs, lens, holes, pow2=scale is None)
+    off = offsets_of(news)
+    q = torch.from_numpy(rng.normal(size=(off[-1], heads * group, dim))).to(dt).cuda()
+    got, lse = kv.cross_attention(cache, q, dev(table), dev(np.int32(lens)), dev(off), scale=scale, return_lse=True,
+                                  max_tokens=max(news))
+    check_cross(Model(cache), got, lse, q, table, lens, off, dim ** -0.5 if scale is None else scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_cross_attention_reads_no_other_tokens(dt):
+    """What lies behind the last token, in other blocks and in holes changes nothing; rows have strides and odd addresses."""
+    rng, heads, dim, bs = np.random.default_rng(33), 2, 64, 32
+    lens, news = [40, 0, 95], [3, 2, 70]
+    cache, table = make(rng, heads, dim, bs, lens)
+    off = offsets_of(news)
+    wide = torch.from_numpy(rng.normal(size=(off[-1], 3, 5, dim + 3))).to(dt).cuda()
+    q = wide[:, 1, :4, 3:]
+    args = dev(table), dev(np.int32(lens)), dev(off)
+    want, lse = kv.cross_attention(cache, q.contiguous(), *args, return_lse=True)
+    for b, n in enumerate(lens):
+        if n % bs:
+            p = int(table[b, n // bs])
+            cache.k[p, :, n % bs:] = 127
+            cache.v[p, :, :, n % bs:] = -127
+    got, other = kv.cross_attention(cache, q, *args, return_lse=True)
+    assert torch.equal(got, want) and torch.equal(lse, other)
+    assert not want[3:5].any() and torch.isneginf(lse[3:5]).all() and torch.isfinite(lse[5:]).all()
+
+
+@pytest.mark.gpu
+def test_cross_attention_equals_attention_of_the_last_rows():
+    """One row a sequence: both see all tokens."""
+    rng = np.random.default_rng(34)
+    for dim, lens in ((128, [3000, 1, 64]), (256, [70000]), (64, [17] * 40)):
+        cache, table = make(rng, 2, dim, 64, lens)
+        q = torch.from_numpy(rng.normal(size=(len(lens), 8, dim))).to(BF16).cuda()
+        args = cache, q, dev(table), dev(np.int32(lens))
+        assert all(torch.equal(a, b) for a, b in zip(kv.attention(*args, return_lse=True), kv.cross_attention(*args, return_lse=True)))
+
+
+# ---------------------------------------------------------------- join
+
+def check_join(parts, lses, rows, got, lse):
+    tokens, heads, dim = got.shape
+    l, o = np.full((len(parts), tokens, heads), -np.inf), np.zeros((len(parts), tokens, heads, dim))
+    for i, (p, s, r) in enumerate(zip(parts, lses, rows)):
+        r = np.arange(tokens) if r is None else r.cpu().numpy()
+        there = (r >= 0) & (r < len(p))
+        l[i, there], o[i, there] = numbers(s)[r[there]], numbers(p)[r[there]]
+    o = np.where(np.isneginf(l)[..., None], 0, o)
+    m = l.max(0)
+    some = np.isfinite(m)
+    x = np.where(some, l - np.where(some, m, 0), -np.inf)
+    w = np.exp(x)
+    total = np.where(some, w.sum(0), 1)
+    want = (w[..., None] * o).sum(0) / total[..., None]
+    e = 2.0 ** -21 + np.where(np.isfinite(x), np.abs(x), 0) * 2.0 ** -23
+    tol = (ROUND[got.dtype] * np.abs(want) + 2 * ((w * e)[..., None] * np.abs(o)).sum(0) / total[..., None]
+           + LEAST[got.dtype] / 2)
+    err = np.abs(numbers(got) - want)
+    assert (err <= tol).all(), float((err - tol).max())
+    if lse is not None:
+        lse, want = numbers(lse), np.where(some, np.where(some, m, 0) + np.log(total), -np.inf)
+        assert (np.isneginf(lse) == ~some).all()
+        t = 2.0 ** -23 * np.abs(want) + 2 * (w * e).max(0) + 2.0 ** -22
+        assert (np.abs(lse[some] - want[some]) <= t[some]).all()
+
+
+def parts_of(rng, count, tokens, heads, dim, dt, some):
+    parts, lses, rows = [], [], []
+    for i in range(count):
+        n, r = tokens, None
+        if some and i % 2:
+            n = max(1, tokens // 2)
+            r = rng.integers(-2, n + 2, tokens)
+            r[rng.random(tokens) < 0.1] = rng.choice([2 ** 31 - 1, -2 ** 31])
+            r = dev(np.int32(r))
+        parts.append(torch.from_numpy(rng.normal(size=(n, heads, dim)) * 10.0 ** rng.uniform(-3, 2)).to(dt).cuda())
+        s = rng.normal(size=(n, heads)) * rng.choice([1, 8, 60]) + rng.choice([0, 300])
+        s[rng.random(s.shape) < 0.2] = -np.inf
+        lses.append(dev(np.float32(s)))
+        rows.append(r)
+    return parts, lses, rows
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("tokens,heads,dim,dt", [(1, 1, 64, BF16), (33, 6, 96, F16), (5, 3, 256, BF16), (70, 2, 7, F16), (3, 1, 2500, BF16),
+                                                 (9, 1, 1, F16), (300, 32, 128, F16)])
+@pytest.mark.parametrize("some", [False, True])
+def test_join(count, tokens, heads, dim, dt, some):
+    rng = np.random.default_rng(count * 100 + tokens)
+    parts, lses, rows = parts_of(rng, count, tokens, heads, dim, dt, some)
+    got, lse = kv.join(parts, lses, rows if some else None, return_lse=True)
+    check_join(parts, lses, rows, got, lse)
+    assert torch.equal(kv.join(parts, lses, rows), got)
+
+
+@pytest.mark.gpu
+def test_join_of_strided_parts_and_of_rows_that_count_for_nothing():
+    rng, dt = np.random.default_rng(41), BF16
+    wide = torch.from_numpy(rng.normal(size=(20, 2, 3, 67))).to(dt).cuda()
+    parts = [wide[:, 0, :, 3:], wide[:, 1, :, :64], wide[:, :, 0, 1:65].transpose(0, 1)[1][:, None].expand(-1, 3, -1)]
+    lses = [dev(np.float32(rng.normal(size=(20, 3)))) for _ in parts]
+    got, lse = kv.join(parts, lses, return_lse=True)
+    check_join(parts, lses, [None] * 3, got, lse)
+    # NaN and infinities in rows that count for nothing
+    bad = [p.clone() for p in parts]
+    for i, x in enumerate((math.nan, math.inf)):
+        lses[i][i::2] = -math.inf
+        bad[i][i::2] = x
+    clean = [torch.where(torch.isfinite(b), b, 0) for b in bad]
+    got, lse = kv.join(bad, lses, return_lse=True)
+    check_join(clean, lses, [None] * 3, got, lse)
+    for s in lses:
+        s[7] = -math.inf
+    out = torch.full((20, 3, 64), 9.0, dtype=dt, device="cuda")
+    assert kv.join(bad, lses, out=out) is out and not out[7].any() and torch.isfinite(out).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_shared_prefix_and_own_tokens_equal_the_whole(dt):
+    """Sequences of two groups that share their group's prompt: the prompt's blocks are read once for a group's rows, each
+    sequence's own behind them, and joined. Against attention over all of it in 64 bits: attention's roundings, those of the two parts (u of
+    each, by weight) and the join's."""
+    rng, heads, group, dim, bs = np.random.default_rng(42), 2, 4, 128, 32
+    shared, each = [10, 3], [5, 4]  # blocks of the prompts, sequences of the groups
+    lens = [s * bs + int(n) for s, c in zip(shared, each) for n in rng.integers(1, 100, c)]
+    cache, full = make(rng, heads, dim, bs, lens)
+    at = 0
+    for s, c in zip(shared, each):
+        full[at:at + c, :s] = full[at, :s]
+        at += c
+    skip = np.repeat(shared, each)
+    own = np.full((len(lens), 5), -1, np.int32)
+    for b, s in enumerate(skip):
+        own[b, :min(5, full.shape[1] - s)] = full[b, s:s + 5]
+    q = torch.from_numpy(rng.normal(size=(len(lens), heads * group, dim))).to(dt).cuda()
+    prefix, l0 = kv.cross_attention(cache, q, dev(full[[0, each[0]], :10].copy()), dev(np.int32([s * bs for s in shared])),
+                                    dev(offsets_of(each)), return_lse=True)
+    rest, l1 = kv.attention(cache, q, dev(own), dev(np.int32(lens) - np.int32(skip * bs)), return_lse=True)
+    got, lse = kv.join([prefix, rest], [l0, l1], return_lse=True)
+    model = Model(cache)
+    o, l, absolute, g = model.attention(numbers(q), full, lens, np.arange(len(lens) + 1), dim ** -0.5)
+    d = g * (dim + 8) * 2.0 ** -24
+    u = ROUND[dt]
+    tol = u * np.abs(o) + (u * (1 + u) + 2.0 ** -11 + 2 * d[..., None] + 2.0 ** -18 + 2.0 ** -17) * absolute
+    assert (np.abs(numbers(got) - o) <= tol).all()
+    assert (np.abs(numbers(lse) - l) <= d + 2.0 ** -19 * (1 + np.abs(l))).all()
+
+
+@pytest.mark.gpu
+def test_graph_of_parts_replays():
+    rng, heads, dim, bs = np.random.default_rng(43), 2, 64, 16
+    cache, table = make(rng, heads, dim, bs, [500, 30, 90])
+    prefix, t, n = dev(table[:1].copy()), dev(table), dev(np.int32([500, 30, 90]))
+    long, off = dev(np.int32([500])), dev(np.int32([0, 3]))
+    q = torch.zeros((3, 8, dim), dtype=F16, device="cuda")
+    rows = dev(np.int32([0, -1, 2]))
+
+    def step():
+        a, l = kv.cross_attention(cache, q, prefix, long, off, return_lse=True)
+        b, m = kv.attention(cache, q, t, n, return_lse=True)
+        return kv.join([a, b], [l, m], [rows, None], return_lse=True)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(5):
+        q.copy_(torch.from_numpy(rng.normal(size=q.shape)))
+        n.copy_(dev(np.int32([rng.integers(1, 500), 30, rng.integers(0, 91)])))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.gpu
+def test_no_rows_and_other_streams():
+    rng = np.random.default_rng(44)
+    cache, table = make(rng, 1, 64, 16, [20])
+    t, n = dev(table), dev(np.int32([20]))
+    q = torch.zeros((0, 2, 64), dtype=BF16, device="cuda")
+    assert kv.cross_attention(cache, q, t, n, dev(np.int32([0, 0]))).shape == (0, 2, 64)
+    got, lse = kv.join([q, q], [q.new_zeros((0, 2)).float()] * 2, return_lse=True)
+    assert got.shape == (0, 2, 64) and lse.shape == (0, 2)
+    empty = kv.join([q], [q.new_zeros((0, 2)).float()], [dev(np.int32([0, 5]))])  # a part without rows
+    assert empty.shape == (2, 2, 64) and not empty.any()
+    # behind work on another stream
+    parts = [torch.from_numpy(rng.normal(size=(6, 2, 64))).to(BF16).cuda() for _ in range(2)]
+    lses = [torch.zeros((6, 2), device="cuda") for _ in range(2)]
+    want, late = kv.join(parts, lses), [torch.zeros_like(p) for p in parts]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    big = torch.randn(4096, 4096, device="cuda")
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            big = big @ big * 1e-4
+        for a, b in zip(late, parts):
+            a.copy_(b)
+        got = kv.join(late, lses)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------- refusals
+
+@pytest.mark.gpu
+def test_refusals():
+    cache = kv.KVCache.empty(4, 2, 64, 16)
+    t, n = torch.zeros((3, 2), dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    q = torch.zeros((3, 4, 64), dtype=BF16, device="cuda")
+    lse = torch.zeros((3, 4), device="cuda")
+    for exc, call in [
+            (TypeError, lambda: kv.cross_attention(cache, q.float(), t, n)),
+            (ValueError, lambda: kv.cross_attention(cache, q[:, :3], t, n)),
+            (ValueError, lambda: kv.cross_attention(cache, q[:2], t, n)),
+            (ValueError, lambda: kv.cross_attention(cache, q, t, n, n)),
+            (ValueError, lambda: kv.cross_attention(cache, q, t, n, out=q[:2])),
+            (RuntimeError, lambda: kv.cross_attention(cache, q, t, n, scale=math.inf)),
+            (ValueError, lambda: kv.join([], [])),
+            (ValueError, lambda: kv.join([q] * 9, [lse] * 9)),
+            (ValueError, lambda: kv.join([q], [])),
+            (ValueError, lambda: kv.join([q], [lse], [])),
+            (ValueError, lambda: kv.join([q[0]], [lse[0]])),
+            (ValueError, lambda: kv.join([q[:, :0]], [lse[:, :0]])),
+            (TypeError, lambda: kv.join([q.float()], [lse])),
+            (TypeError, lambda: kv.join([q, q.half()], [lse, lse])),
+            (ValueError, lambda: kv.join([q, q[..., :32]], [lse, lse])),
+            (ValueError, lambda: kv.join([q, q[:2]], [lse, lse[:2]])),
+            (ValueError, lambda: kv.join([q.transpose(1, 2)], [lse])),
+            (ValueError, lambda: kv.join([q.cpu()], [lse.cpu()])),
+            (ValueError, lambda: kv.join([q, q.cpu()], [lse, lse])),
+            (TypeError, lambda: kv.join([q], [lse.half()])),
+            (ValueError, lambda: kv.join([q], [lse[:2]])),
+            (ValueError, lambda: kv.join([q], [lse.t().contiguous().t()])),
+            (TypeError, lambda: kv.join([q], [lse], [n.long()])),
+            (ValueError, lambda: kv.join([q, q], [lse, lse], [None, n[:2]])),
+            (ValueError, lambda: kv.join([q], [lse], [n[:0].view(0, 1)])),
+            (ValueError, lambda: kv.join([q], [lse], out=q[:2]))]:
+        with pytest.raises(exc):
+            call()
+
+
+def test_entries_refuse_before_any_device_work(capfd):
+    """Pointers that are never followed: every call is refused on the host."""
+    L, p = kv._bind(), 1 << 20
+    for change in ({"k": None}, {"dim": 100}, {"table": None}, {"seqs": 0}, {"max_tokens": 6}, {"data": None}, {"heads": 3}, {"dtype": 0}):
+        c, b, r = fake(**change)
+        assert L.dance_kv_cross_attention(c, b, r, 1.0, p, None, p, 1 << 40, None) == -1
+        assert "dance_kv_cross_attention" in capfd.readouterr().err
+    c, b, r = fake(seqs=1, table_width=5000, tokens=1, max_tokens=1)
+    r.heads = 2
+    need = L.dance_kv_cross_attention_work(c, b, 2)
+    assert need > 0 and L.dance_kv_cross_attention_work(c, b, 3) == 0 and L.dance_kv_cross_attention_work(c, b, 0) == 0
+    for at, size in ((None, need), (p, need - 1), (p | 8, need)):
+        assert L.dance_kv_cross_attention(c, b, r, 1.0, p, None, at, size, None) == -1
+    assert L.dance_kv_cross_attention(c, b, r, math.nan, p, None, p, need, None) == -1
+    assert L.dance_kv_cross_attention(c, b, r, 1.0, None, None, p, need, None) == -1
+
+    def part(data=p, lse=p, rows=None, tokens=5):
+        return kv.DanceKvPart(data, 256, 64, lse, rows, tokens)
+
+    def join(parts, count=None, tokens=5, heads=4, dim=64, dtype=3, out=p):
+        a = (kv.DanceKvPart * max(1, len(parts)))(*parts) if parts is not None else None
+        return L.dance_kv_join(a, len(parts or []) if count is None else count, tokens, heads, dim, dtype, out, None, None)
+
+    ok = part()
+    for args in ([None], [[]], [[ok] * 9], [[part(None)]], [[part(p | 1)]], [[ok, part(lse=None)]], [[part(tokens=4)]],
+                 [[part(rows=p, tokens=1 << 31)]]):
+        assert join(*args) == -1
+    for change in ({"heads": 0}, {"heads": 1 << 16}, {"dim": 0}, {"dim": 1 << 17}, {"dtype": 1}, {"out": None}, {"out": p | 1},
+                   {"tokens": 4}):
+        assert join([ok, ok], **change) == -1
+    assert join([part(tokens=1 << 30)], tokens=1 << 30) == -1  # 2^32 rows
+    assert join([part(None, None, None, 0)], tokens=0, out=None) == 0
+    assert capfd.readouterr().err.count("dance_kv_join") == 8 + 8 + 1
