@@ -43,37 +43,38 @@ __device__ __forceinline__ uint32_t block_sum(uint32_t x, uint32_t* lds) {
 
 // Workgroups of old rows change the counts, by a row's children less one: where a
 // row goes on as one, in whatever slot, nothing is to be counted. Those of new
-// rows copy them.
+// rows copy them, behind the others, whose atomics take longer.
 __global__ __launch_bounds__(kThreads) void k_fork(Pages p, Table t, const int32_t* __restrict__ parents, uint32_t fresh,
                                                    uint32_t runs, int32_t* __restrict__ table, int32_t* __restrict__ lengths) {
   __shared__ uint32_t lds[kWaves];
   const uint32_t run = blockIdx.x % runs, row = blockIdx.x / runs;
   const uint32_t e0 = run * kRun + threadIdx.x;
-  if (row < fresh) {
-    const int32_t from = parents[row];
+  if (row >= t.seqs) {
+    const uint32_t to = row - t.seqs;
+    const int32_t from = parents[to];
     const bool ok = (uint32_t)from < t.seqs;
     const int32_t* const src = t.table + (size_t)(ok ? from : 0) * t.width;
-    int32_t* const dst = table + (size_t)row * t.width;
+    int32_t* const dst = table + (size_t)to * t.width;
     int32_t x[kEntries];
 #pragma unroll
-    for (uint32_t i = 0; i < kEntries; ++i) x[i] = ok && e0 + i * kThreads < t.width ? src[e0 + i * kThreads] : -1;
+    for (uint32_t i = 0; i < kEntries; ++i) x[i] = src[min(e0 + i * kThreads, t.width - 1u)];
 #pragma unroll
     for (uint32_t i = 0; i < kEntries; ++i)
-      if (e0 + i * kThreads < t.width) dst[e0 + i * kThreads] = x[i];
-    if (run == 0 && threadIdx.x == 0) lengths[row] = ok ? t.lengths[from] : 0;
+      if (e0 + i * kThreads < t.width) dst[e0 + i * kThreads] = ok ? x[i] : -1;
+    if (run == 0 && threadIdx.x == 0) lengths[to] = ok ? t.lengths[from] : 0;
     return;
   }
-  const uint32_t old = row - fresh;
+  const int32_t* const src = t.table + (size_t)row * t.width;
+  int32_t x[kEntries];
+#pragma unroll
+  for (uint32_t i = 0; i < kEntries; ++i) x[i] = src[min(e0 + i * kThreads, t.width - 1u)];
   uint32_t mine = 0;
-  for (uint32_t i = threadIdx.x; i < fresh; i += kThreads) mine += (uint32_t)parents[i] == old ? 1u : 0u;
+  for (uint32_t i = threadIdx.x; i < fresh; i += kThreads) mine += (uint32_t)parents[i] == row ? 1u : 0u;
   const int32_t more = (int32_t)block_sum(mine, lds) - 1;
   if (more == 0) return;
-  const int32_t* const src = t.table + (size_t)old * t.width;
 #pragma unroll
-  for (uint32_t i = 0; i < kEntries; ++i) {
-    const int32_t x = e0 + i * kThreads < t.width ? src[e0 + i * kThreads] : -1;
-    if ((uint32_t)x < p.blocks) atomicAdd(p.refs + x, more);
-  }
+  for (uint32_t i = 0; i < kEntries; ++i)
+    if (e0 + i * kThreads < t.width && (uint32_t)x[i] < p.blocks) atomicAdd(p.refs + x[i], more);
 }
 
 // ------------------------------------------------------------- reserve
@@ -107,67 +108,89 @@ __device__ __forceinline__ Growth growth(const Table& t, const int32_t* __restri
   return g;
 }
 
-// What there is and what is asked for: a wave looks at kFree blocks, or at one sequence. Nothing
-// that the other waves read is changed here.
+// A wave's kFree blocks from `at` * kFree: a word of free ones in each of its first lanes, and their number.
+struct Free {
+  uint64_t word;
+  uint32_t count;
+};
+__device__ __forceinline__ Free free_of(const Pages& p, uint32_t at, uint32_t lane) {
+  int32_t r[kWords];
+  const uint32_t b0 = at * kFree + lane;
+#pragma unroll
+  for (uint32_t i = 0; i < kWords; ++i) r[i] = p.refs[min(b0 + i * 64, p.blocks - 1u)];
+  Free f{0, 0};
+#pragma unroll
+  for (uint32_t i = 0; i < kWords; ++i) {
+    const uint64_t mask = __ballot(r[i] == 0 && b0 + i * 64 < p.blocks);
+    f.count += (uint32_t)__popcll(mask);
+    if (lane == i) f.word = mask;
+  }
+  return f;
+}
+
+// The places j0 .. of a sequence that need a block, as far as 64 of them go; without the partly filled one.
+__device__ __forceinline__ uint64_t fresh_of(const Pages& p, const Growth& g, const int32_t* row, uint32_t j0, uint32_t lane) {
+  const uint32_t j = j0 + lane;
+  const bool asked = j < g.end && !(g.partly && j == g.first);
+  const int32_t x = asked ? row[j] : -1;
+  const bool valid = (uint32_t)x < p.blocks;
+  return __ballot(asked && (!valid || p.refs[valid ? x : 0] > 1));
+}
+
+// What there is and what is asked for: a wave looks at kFree blocks, a workgroup at one sequence. Nothing
+// that the others read is changed here.
 __global__ __launch_bounds__(kThreads) void k_needs(Pages p, Table t, const int32_t* __restrict__ upto, Needs n) {
-  const uint32_t lane = threadIdx.x & 63u;
-  const uint32_t at = blockIdx.x * kWaves + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  if (at < n.counts) {
-    int32_t r[kWords];
-    const uint32_t b0 = at * kFree + lane;
-#pragma unroll
-    for (uint32_t i = 0; i < kWords; ++i) r[i] = b0 + i * 64 < p.blocks ? p.refs[b0 + i * 64] : 1;
-    uint64_t mine = 0;
-    uint32_t sum = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kWords; ++i) {
-      const uint64_t mask = __ballot(r[i] == 0);
-      sum += (uint32_t)__popcll(mask);
-      if (lane == i) mine = mask;
-    }
-    if (lane < kWords) n.free[(size_t)at * kWords + lane] = mine;
-    if (lane == 0) n.count[at] = sum;
+  __shared__ uint32_t lds[kWaves], most[kWaves];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+  if (blockIdx.x >= t.seqs) {
+    const uint32_t at = (blockIdx.x - t.seqs) * kWaves + wave;
+    if (at >= n.counts) return;
+    const Free f = free_of(p, at, lane);
+    if (lane < kWords) n.free[(size_t)at * kWords + lane] = f.word;
+    if (lane == 0) n.count[at] = f.count;
     return;
   }
-  const uint32_t b = at - n.counts;
-  if (b >= t.seqs) return;
+  const uint32_t b = blockIdx.x;
   const Growth g = growth(t, upto, b, p.bsh);
+  if (!g.grows) {
+    if (tid == 0) n.need[b] = 0;
+    return;
+  }
+  const int32_t* const row = t.table + (size_t)b * t.width;
   uint32_t need = 0;
-  if (g.grows) {
-    const int32_t* const row = t.table + (size_t)b * t.width;
-    for (uint32_t j0 = g.first; j0 < g.end; j0 += 64) {
-      const uint32_t j = j0 + lane;
-      const int32_t x = j < g.end ? row[j] : -1;
-      const bool valid = (uint32_t)x < p.blocks;
-      const bool many = valid && p.refs[valid ? x : 0] > 1;
-      const bool part = g.partly && j == g.first;
-      uint64_t mask = __ballot(j < g.end && (part ? many : many || !valid));
-      if (g.partly && j0 == g.first && (mask & 1u)) {
-        // The partly filled block has other owners. Those that grow in this call too will not write it.
-        const int32_t block = __builtin_amdgcn_readfirstlane(x);
-        uint32_t owners = 0, last = 0;
-        for (uint32_t c = lane; c < t.seqs; c += 64) {
-          const Growth o = growth(t, upto, c, p.bsh);
-          if (o.grows && o.partly && t.table[(size_t)c * t.width + o.first] == block) {
-            ++owners;
-            last = c;
-          }
-        }
-#pragma unroll
-        for (int i = 1; i < 64; i <<= 1) {
-          owners += (uint32_t)__shfl_xor((int)owners, i);
-          last = max(last, (uint32_t)__shfl_xor((int)last, i));
-        }
-        if (last == b && (int32_t)owners == p.refs[block]) {
-          mask &= ~1ull;
-          need |= kLast;
+  bool last = false, shared = false;
+  if (g.partly) {
+    const int32_t block = row[g.first];
+    const int32_t refs = (uint32_t)block < p.blocks ? p.refs[block] : 0;
+    shared = refs > 1;
+    if (shared) {
+      // The partly filled block has other owners. If all of them grow in this call, the last one need not copy it.
+      uint32_t owners = 0, top = 0;
+      for (uint32_t c = tid; c < t.seqs; c += kThreads) {
+        const Growth o = growth(t, upto, c, p.bsh);
+        if (o.grows && o.partly && t.table[(size_t)c * t.width + o.first] == block) {
+          ++owners;
+          top = c;
         }
       }
-      need += (uint32_t)__popcll(mask);
-      if (lane == 0) n.fresh[(size_t)b * n.words + (j0 - g.first) / 64] = mask;
+      owners = block_sum(owners, lds);
+#pragma unroll
+      for (int i = 1; i < 64; i <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, i));
+      if (lane == 0) most[wave] = top;
+      __syncthreads();
+#pragma unroll
+      for (uint32_t w = 0; w < kWaves; ++w) top = max(top, most[w]);
+      last = top == b && (int32_t)owners == refs;
     }
   }
-  if (lane == 0) n.need[b] = need;
+  for (uint32_t w = wave; g.first + w * 64 < g.end; w += kWaves) {
+    uint64_t mask = fresh_of(p, g, row, g.first + w * 64, lane);
+    if (w == 0 && shared && !last) mask |= 1ull;
+    need += lane == 0 ? (uint32_t)__popcll(mask) : 0u;
+    if (lane == 0) n.fresh[(size_t)b * n.words + w] = mask;
+  }
+  need = block_sum(need, lds);
+  if (tid == 0) n.need[b] = need | (last ? kLast : 0u);
 }
 
 // The bit of a word with `rank` set ones below it; the word has more than that.
@@ -182,6 +205,45 @@ __device__ __forceinline__ uint32_t select_bit(uint64_t w, uint32_t rank) {
     w = up ? w >> half : w;
   }
   return at;
+}
+
+// The free block with `rank` others before it in a run of kFree, by its words.
+template <typename P>
+__device__ __forceinline__ uint32_t block_of(P words, uint32_t rank) {
+  uint64_t word[kWords], mine = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kWords; ++i) word[i] = words[i];
+  uint32_t which = kWords;
+#pragma unroll
+  for (uint32_t i = 0; i < kWords; ++i) {
+    const uint32_t ones = (uint32_t)__popcll(word[i]);
+    if (which == kWords) {
+      if (rank < ones) {
+        which = i;
+        mine = word[i];
+      } else {
+        rank -= ones;
+      }
+    }
+  }
+  return which * 64 + select_bit(mine, rank);
+}
+
+// Gives a sequence the block for its `rank`-th fresh place.
+template <typename P>
+__device__ __forceinline__ void give(const Pages& p, int32_t* row, uint32_t first, bool partly, P fresh, uint32_t rank, uint32_t block,
+                                     int32_t* src, int32_t* dst) {
+  uint32_t w = 0;
+  for (uint32_t ones; rank >= (ones = (uint32_t)__popcll(fresh[w])); ++w) rank -= ones;
+  const uint32_t j = first + w * 64 + select_bit(fresh[w], rank);
+  const int32_t old = row[j];
+  row[j] = (int32_t)block;
+  p.refs[block] = 1;
+  if ((uint32_t)old < p.blocks) atomicAdd(p.refs + old, -1);
+  if (partly && j == first) {
+    *src = old;
+    *dst = (int32_t)block;
+  }
 }
 
 // A workgroup for each sequence: the needs before it say which free blocks are
@@ -235,38 +297,96 @@ __global__ __launch_bounds__(kThreads) void k_give(Pages p, Table t, const int32
       for (uint32_t step = kThreads / 2; step; step >>= 1)
         if (upper[at + step - 1] <= r) at += step;
       r -= at ? upper[at - 1] : 0u;
-      const uint64_t* const words = n.free + (size_t)(c0 + at) * kWords;
-      uint64_t word[kWords], bits = 0;
-#pragma unroll
-      for (uint32_t i = 0; i < kWords; ++i) word[i] = words[i];
-      uint32_t which = kWords;
-#pragma unroll
-      for (uint32_t i = 0; i < kWords; ++i) {
-        const uint32_t ones = (uint32_t)__popcll(word[i]);
-        if (which == kWords) {
-          if (r < ones) {
-            which = i;
-            bits = word[i];
-          } else {
-            r -= ones;
-          }
-        }
-      }
-      const uint32_t block = ((c0 + at) * kWords + which) * 64 + select_bit(bits, r);
-      uint32_t k = rank - before, w = 0;  // its place
-      for (uint32_t ones; k >= (ones = (uint32_t)__popcll(fresh[w])); ++w) k -= ones;
-      const uint32_t j = g.first + w * 64 + select_bit(fresh[w], k);
-      const int32_t old = row[j];
-      row[j] = (int32_t)block;
-      p.refs[block] = 1;
-      if ((uint32_t)old < p.blocks) atomicAdd(p.refs + old, -1);
-      if (g.partly && j == g.first) {
-        src[b] = old;
-        dst[b] = (int32_t)block;
-      }
+      const uint32_t block = (c0 + at) * kFree + block_of(n.free + (size_t)(c0 + at) * kWords, r);
+      give(p, row, g.first, g.partly, fresh, rank - before, block, src + b, dst + b);
     }
     base += all;
     if (c0 + kThreads >= n.counts) break;
+  }
+}
+
+// Both in one workgroup, for up to kSmall runs of blocks and 64 sequences of up to kSmallWords words: a decoding step's
+// batch. Its bits stay in LDS. Measured, in a graph, with this and with two launches: 64 sequences over 3979 blocks 4.7 and 6.9
+// us, 32 over 254 that all share a block 6.5 and 8.4; a launch is also 3 us of the host.
+constexpr uint32_t kSmall = 16, kSmallWords = 16;
+__global__ __launch_bounds__(64 * kSmall) void k_reserve(Pages p, Table t, const int32_t* __restrict__ upto, uint32_t counts,
+                                                         int32_t* __restrict__ now, int32_t* __restrict__ src,
+                                                         int32_t* __restrict__ dst) {
+  __shared__ uint64_t free[kSmall][kWords], fresh[64][kSmallWords];
+  __shared__ uint32_t count[kSmall], need[64];
+  const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  // Lane b of every wave knows sequence b.
+  Growth g{};
+  int32_t block = -1, refs = 0;
+  if (lane < t.seqs) {
+    g = growth(t, upto, lane, p.bsh);
+    if (g.grows && g.partly) block = t.table[(size_t)lane * t.width + g.first];
+    if ((uint32_t)block < p.blocks) refs = p.refs[block];
+  }
+  if (wave < counts) {
+    const Free f = free_of(p, wave, lane);
+    if (lane < kWords) free[wave][lane] = f.word;
+    if (lane == 0) count[wave] = f.count;
+  } else if (lane == 0) {
+    count[wave] = 0;
+  }
+  // Of the owners of a partly filled block that all grow, the last one need not copy it.
+  bool copies = refs > 1, last = false;
+  for (uint64_t rest = __ballot(copies); rest;) {
+    const int32_t one = __builtin_amdgcn_readlane(block, __builtin_ctzll(rest));
+    const uint64_t same = __ballot(block == one);
+    if (block == one && (int32_t)__popcll(same) == refs && (same >> lane) == 1ull) {
+      last = true;
+      copies = false;
+    }
+    rest &= ~same;
+  }
+  for (uint32_t b = wave; b < t.seqs; b += kSmall) {
+    const Growth o{0, 0, true, (uint32_t)__builtin_amdgcn_readlane((int)g.first, (int)b),
+                   (uint32_t)__builtin_amdgcn_readlane((int)(g.grows ? g.end : 0u), (int)b),
+                   (bool)__builtin_amdgcn_readlane((int)g.partly, (int)b)};
+    const uint64_t tail = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)copies, (int)b);
+    uint32_t sum = 0;
+    for (uint32_t w = 0; o.first + w * 64 < o.end; ++w) {
+      const uint64_t mask = fresh_of(p, o, t.table + (size_t)b * t.width, o.first + w * 64, lane) | (w ? 0ull : tail);
+      sum += (uint32_t)__popcll(mask);
+      if (lane == 0) fresh[b][w] = mask;
+    }
+    if (lane == 0) need[b] = sum;
+  }
+  __syncthreads();
+  const uint32_t mine = lane < t.seqs ? need[lane] : 0u, have = lane < kSmall ? count[lane] : 0u;
+  uint32_t upper = mine, cum = have;
+#pragma unroll
+  for (uint32_t i = 1; i < 64; i <<= 1) {
+    const uint32_t x = (uint32_t)__shfl_up((int)upper, i), y = (uint32_t)__shfl_up((int)cum, i);
+    upper += lane >= i ? x : 0u;
+    cum += lane >= i ? y : 0u;
+  }
+  const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)cum, 63);
+  const bool served = g.grows && (upper <= total || !(mine || last));
+  if (wave == 0 && lane < t.seqs) {
+    now[lane] = served ? g.upto : g.upto <= g.len ? g.len : 0;
+    if (served) t.lengths[lane] = g.upto;
+    if (!(served && copies)) src[lane] = dst[lane] = -1;
+  }
+  for (uint32_t b = wave; b < t.seqs; b += kSmall) {
+    const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)(served ? mine : 0u), (int)b);
+    const uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)(upper - mine), (int)b);
+    const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)g.first, (int)b);
+    const bool partly = __builtin_amdgcn_readlane((int)g.partly, (int)b);
+    for (uint32_t k0 = 0; k0 < n; k0 += 64) {
+      uint32_t rank = before + k0 + lane, run = 0, below = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < kSmall; ++i) {
+        const uint32_t c = (uint32_t)__builtin_amdgcn_readlane((int)cum, (int)i);
+        run += rank >= c ? 1u : 0u;
+        below = rank >= c ? c : below;
+      }
+      if (k0 + lane < n)
+        give(p, t.table + (size_t)b * t.width, first, partly, fresh[b], k0 + lane, run * kFree + block_of(free[run], rank - below),
+             src + b, dst + b);
+    }
   }
 }
 
@@ -283,13 +403,16 @@ __global__ __launch_bounds__(kThreads) void k_release(Pages p, Table t, const in
     if (run == 0 && threadIdx.x == 0) t.lengths[b] = len;
   }
   int32_t* const row = t.table + (size_t)b * t.width;
+  int32_t x[kEntries];
+  const uint32_t j0 = run * kRun + threadIdx.x;
+#pragma unroll
+  for (uint32_t i = 0; i < kEntries; ++i) x[i] = row[min(j0 + i * kThreads, t.width - 1u)];
 #pragma unroll
   for (uint32_t i = 0; i < kEntries; ++i) {
-    const uint32_t j = run * kRun + i * kThreads + threadIdx.x;
-    if (j >= t.width || (j >= from && j < to)) continue;
-    const int32_t x = row[j];
-    if (x != -1) row[j] = -1;
-    if ((uint32_t)x < p.blocks) atomicAdd(p.refs + x, -1);
+    const uint32_t j = j0 + i * kThreads;
+    if (j >= t.width || (j >= from && j < to) || x[i] == -1) continue;
+    row[j] = -1;
+    if ((uint32_t)x[i] < p.blocks) atomicAdd(p.refs + x[i], -1);
   }
 }
 
@@ -395,6 +518,7 @@ bool too_many(uint64_t workgroups) { return workgroups * kThreads > 0xFFFFFFFFul
 
 struct Sizes {
   uint64_t counts, words, fresh, need, count, all;  // entries, words of a sequence, byte offsets, bytes
+  bool small;                                        // one workgroup's LDS holds them
 };
 Sizes reserve_sizes(const DanceKvPages* p, uint32_t seqs, uint32_t width) {
   Sizes z;
@@ -403,7 +527,8 @@ Sizes reserve_sizes(const DanceKvPages* p, uint32_t seqs, uint32_t width) {
   z.fresh = z.counts * kWords * 8;
   z.need = z.fresh + z.words * seqs * 8;
   z.count = z.need + (uint64_t)seqs * 4;
-  z.all = z.count + z.counts * 4;
+  z.small = z.counts <= kSmall && seqs <= 64 && z.words <= kSmallWords;
+  z.all = z.small ? 0 : z.count + z.counts * 4;
   return z;
 }
 
@@ -456,15 +581,19 @@ int dance_kv_reserve(const DanceKvPages* pages, int32_t* table, int32_t* lengths
   if (!why && ((uint64_t)seqs * width > 0x7FFFFFFFull)) why = "a table must have fewer than 2^31 entries";
   if (why) KV_ERR("dance_kv_reserve", "%s", why);
   const Sizes z = reserve_sizes(pages, seqs, width);
+  const Table t{table, lengths, seqs, width};
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (z.small) {
+    hipLaunchKernelGGL(k_reserve, dim3(1), dim3(64 * kSmall), 0, st, pages_args(pages), t, upto, (uint32_t)z.counts, now, src, dst);
+    return launched("dance_kv_reserve");
+  }
   if (!work || work_bytes < z.all || !aligned(work, 16))
     KV_ERR("dance_kv_reserve", "work must hold %zu bytes, aligned to 16", (size_t)z.all);
-  const uint64_t first = (z.counts + seqs + kWaves - 1) / kWaves;
+  const uint64_t first = seqs + (z.counts + kWaves - 1) / kWaves;
   if (too_many(first) || too_many(seqs)) KV_ERR("dance_kv_reserve", "batch is too large for one launch");
   char* const w = static_cast<char*>(work);
   const Needs n{reinterpret_cast<uint64_t*>(w), reinterpret_cast<uint64_t*>(w + z.fresh), reinterpret_cast<uint32_t*>(w + z.count),
                 reinterpret_cast<uint32_t*>(w + z.need), (uint32_t)z.counts, (uint32_t)z.words};
-  const Table t{table, lengths, seqs, width};
-  const hipStream_t st = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(k_needs, dim3((uint32_t)first), dim3(kThreads), 0, st, pages_args(pages), t, upto, n);
   hipLaunchKernelGGL(k_give, dim3(seqs), dim3(kThreads), 0, st, pages_args(pages), t, upto, n, now, src, dst);
   return launched("dance_kv_reserve");

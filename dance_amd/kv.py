@@ -383,25 +383,29 @@ def join(parts, lses, rows=None, *, out=None, return_lse=False):
     if heads < 1 or dim < 1:
         raise ValueError("parts must have heads and dimensions")
     tokens, args = None, []
-    for i, (x, lse) in enumerate(zip(parts, lses)):
-        at = rows[i] if rows is not None else None
-        if x.ndim != 3 or x.shape[1:] != first.shape[1:]:
+    for i in range(count):
+        x, lse, at = parts[i], lses[i], rows[i] if rows is not None else None
+        shape, strides = x.shape, x.stride()
+        n = shape[0]
+        if shape != (n, heads, dim):
             raise ValueError("parts must have one number of heads and dimensions")
         if x.dtype != dtype:
             raise TypeError("parts must have one type")
-        if x.device != device or x.stride(2) != 1 and dim > 1:
+        if x.device != device or strides[2] != 1 and dim > 1:
             raise ValueError("parts must be on one device, with adjacent dimensions")
         if lse.dtype != torch.float32:
             raise TypeError("lses must be float32")
-        if lse.shape != x.shape[:2] or lse.device != device or not lse.is_contiguous():
+        if lse.shape != (n, heads) or lse.device != device or not lse.is_contiguous():
             raise ValueError("lses must be contiguous, [tokens, heads], on the parts' device")
+        own = 0
         if at is not None:
             _ints("rows", at, at.shape[:1], device)
-        n = x.shape[0] if at is None else at.shape[0]
-        if tokens is not None and n != tokens:
+            own, n = at.data_ptr(), at.shape[0]
+        if tokens is None:
+            tokens = n
+        elif n != tokens:
             raise ValueError("parts, or their rows, must have one number of tokens")
-        tokens = n
-        args.append(_PART.pack(x.data_ptr(), x.stride(0), x.stride(1), lse.data_ptr(), _ptr(at) or 0, x.shape[0]))
+        args.append(_PART.pack(x.data_ptr(), strides[0], strides[1], lse.data_ptr(), own, shape[0]))
     shape = (tokens, heads, dim)
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=device)
@@ -432,8 +436,10 @@ def fork(pages, table, lengths, parents):
     if new == 0:
         raise ValueError("parents must be [new sequences]")
     _ints("parents", parents, (new,), pages.device)
-    new_table = torch.empty((new, width), dtype=torch.int32, device=pages.device)
-    new_lengths = torch.empty(new, dtype=torch.int32, device=pages.device)
+    if new == seqs:
+        new_table, new_lengths = torch.empty_like(table), torch.empty_like(lengths)
+    else:
+        new_table, new_lengths = table.new_empty((new, width)), lengths.new_empty(new)
     _call("fork", pages, table.data_ptr(), lengths.data_ptr(), seqs, width, parents.data_ptr(), new, new_table.data_ptr(),
           new_lengths.data_ptr())
     return new_table, new_lengths
@@ -447,7 +453,7 @@ def reserve(pages, table, lengths, upto):
     is written. Sequences and their places take the free blocks in ascending order."""
     seqs, width = _table(pages, table, lengths)
     _ints("upto", upto, (seqs,), pages.device)
-    now, src, dst = torch.empty((3, seqs), dtype=torch.int32, device=pages.device).unbind(0)
+    now, src, dst = table.new_empty((3, seqs)).unbind(0)
     size = _fast["reserve_work"](pages._bytes, seqs, width)
     work = _work(pages, size)
     _call("reserve", pages, table.data_ptr(), lengths.data_ptr(), seqs, width, upto.data_ptr(), now.data_ptr(), src.data_ptr(),

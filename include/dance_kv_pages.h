@@ -44,7 +44,7 @@ int dance_kv_fork(const DanceKvPages *pages, const int32_t *table, const int32_t
  * Where served, lengths[b] becomes upto[b] and so does now[b]; where not, lengths[b]
  * stays and now[b] is 0, with which an append writes nothing and attention
  * sees nothing. Where upto[b] <= lengths[b] nothing happens and now[b] is lengths[b]. `work` holds at
- * least dance_kv_reserve_work() bytes, aligned to 16, as dance_kv_attention's. */
+ * least dance_kv_reserve_work() bytes, aligned to 16 (null where that is 0), as dance_kv_attention's. */
 int dance_kv_reserve(const DanceKvPages *pages, int32_t *table, int32_t *lengths, uint32_t seqs, uint32_t width,
                      const int32_t *upto, int32_t *now, int32_t *src, int32_t *dst, void *work, size_t work_bytes,
                      void *stream);

@@ -144,7 +144,10 @@ def owners(rng, seqs, width, bs, blocks, most, holes=0, pinned=0):
 # sequences, width, block tokens, blocks, longest, holes, pinned
 POOLS = [(1, 1, 16, 1, 16, 0, 0), (1, 3, 128, 5, 300, 0, 1), (5, 7, 16, 40, 100, 0, 2), (8, 9, 32, 64, 200, 6, 0),
          (33, 5, 64, 130, 300, 0, 3), (70, 70, 16, 1500, 900, 20, 4), (3, 1500, 16, 5000, 20000, 5, 0),
-         (300, 4, 16, 1025, 60, 0, 0), (9, 130, 16, 300000, 2000, 0, 9)]
+         (300, 4, 16, 1025, 60, 0, 0), (9, 130, 16, 300000, 2000, 0, 9),
+         # at the ends of what one workgroup takes, and beyond each
+         (64, 1024, 16, 16384, 2000, 9, 5), (65, 1024, 16, 16384, 2000, 9, 5), (64, 1025, 16, 16384, 2000, 9, 5),
+         (64, 1024, 16, 16385, 2000, 9, 5), (64, 3, 16, 70, 40, 0, 0)]
 
 
 @pytest.mark.gpu
@@ -627,9 +630,10 @@ def test_entries_refuse_before_any_device_work(capfd):
                   (L.dance_kv_reserve, [bad, p, p, 2, 3, p, p, p, p, p, 1 << 30, None]),
                   (L.dance_kv_release, [bad, p, p, 2, 3, p, p, None])]
         assert L.dance_kv_reserve_work(bad, 2, 3) == 0
-    ok = pages()
-    need = L.dance_kv_reserve_work(ok, 2, 3)
-    assert need == 16 * 8 + 2 * 8 + 2 * 4 + 4
+    ok, large = pages(), pages(blocks=1 << 20)
+    assert L.dance_kv_reserve_work(ok, 2, 3) == 0  # one workgroup's
+    need = L.dance_kv_reserve_work(large, 2, 3)
+    assert need == (1 << 17) + 2 * 8 + 2 * 4 + 4096
     for seqs, width in ((0, 3), (2, 0), (2, 1 << 28)):
         calls += [(L.dance_kv_fork, [ok, p, p, seqs, width, p, 2, p + 64, p + 64, None]),
                   (L.dance_kv_reserve, [ok, p, p, seqs, width, p, p, p, p, p, 1 << 30, None]),
@@ -643,11 +647,11 @@ def test_entries_refuse_before_any_device_work(capfd):
               (L.dance_kv_fork, [ok, p, p, 2, 3, p, 2, p + 64, p, None]),
               (L.dance_kv_fork, [ok, p, p, 1 << 24, 1 << 10, p, 2, p + 64, p + 64, None])]  # more threads than a launch has
     for i in (1, 2, 5, 6, 7, 8, 9):
-        args = [ok, p, p, 2, 3, p, p, p, p, p, need, None]
+        args = [large, p, p, 2, 3, p, p, p, p, p, need, None]
         args[i] = None
         calls.append((L.dance_kv_reserve, args))
-    calls += [(L.dance_kv_reserve, [ok, p, p, 2, 3, p, p, p, p, p, need - 1, None]),
-              (L.dance_kv_reserve, [ok, p, p, 2, 3, p, p, p, p, p + 8, need, None]),
+    calls += [(L.dance_kv_reserve, [large, p, p, 2, 3, p, p, p, p, p, need - 1, None]),
+              (L.dance_kv_reserve, [large, p, p, 2, 3, p, p, p, p, p + 8, need, None]),
               (L.dance_kv_reserve, [ok, p, p, 1 << 20, 1 << 12, p, p, p, p, p, 1 << 50, None]),
               (L.dance_kv_release, [ok, None, p, 2, 3, p, p, None]), (L.dance_kv_release, [ok, p, None, 2, 3, p, p, None])]
     c = fake()[0]
