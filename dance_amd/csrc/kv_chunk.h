@@ -3,8 +3,8 @@
 //
 // A wave takes 32 rows, a workgroup W waves. The codes of 64 tokens become
 // f16 in LDS once per workgroup (the conversion is then a tenth of a wave's
-// instructions), two tiles deep, so that one barrier a tile is enough: while a tile is
-// computed the next one's codes are in registers and the one after is on its way.
+// instructions), two tiles deep, so that one barrier a tile is enough: around a tile's products the next one's codes
+// go from registers to LDS and those of the one after set out.
 // Products with 32x32x16 f16 MFMAs, S' = K Q' and O' += V' P'. Result
 // register i of S' is token 8 (i / 4) + 4 (lane / 32) + i % 4 of 32; eight
 // registers are one group of 16 tokens, which has one scale, and in their order the weights'
@@ -12,11 +12,14 @@
 // operand wants: within 16 tokens 0-3, 8-11, 4-7, 12-15, a swap of words.
 //
 // Bound by the softmax's and the conversion's vector instructions and the matrix units in turn: two chunks of
-// 2048 tokens over 6,000 to 10,000, 8 kv heads of 4, 128 dimensions (491 GFLOP), 528 us, 930 TFLOP/s; a
-// large f16 product reaches 1370. Vector instructions are 50 %, matrix instructions 38 % of the time.
+// 2048 tokens over 6,000 to 10,000, 8 kv heads of 4, 128 dimensions (491 GFLOP), 513 us, 957 TFLOP/s; a
+// large f16 product reaches 1370. Vector instructions are 54 %, matrix instructions 42 % of the time.
 #pragma once
 
-constexpr int chunk_occ(int d) { return d <= 128 ? 2 : 1; }  // waves per SIMD, by registers
+// Waves per SIMD, by registers. At 64 dimensions, where a tile has half the products for as much softmax, more waves
+// hide more: 8 sequences of 300 rows over 3000 tokens (8 kv heads of 4, bf16) take 104 us with three, 117 with two; four
+// spill.
+constexpr int chunk_occ(int d) { return d <= 64 ? 3 : d <= 128 ? 2 : 1; }
 
 typedef float f16_t __attribute__((ext_vector_type(16)));
 
@@ -39,9 +42,13 @@ __global__ __launch_bounds__(64 * W)
   constexpr uint32_t kChunks = 4 * D;     // 16-byte pieces of a tile's key codes, and of its value codes
   constexpr int CN = (kChunks + 64 * W - 1) / (64 * W);
   constexpr uint32_t kRows = W * 32;
+  // The next tile's codes go to LDS ahead of a tile's products, which hide the conversion; with one wave a SIMD, behind
+  // them (two chunks of 1024 rows over 4000 tokens: at 128 dimensions 5 % less, at 192 and 256 21 and 7 % more).
+  constexpr bool kAhead = D <= 128;
   __shared__ __attribute__((aligned(16))) char sk[2][64 * KST];
   __shared__ __attribute__((aligned(16))) char sv[2][D * VST];
-  __shared__ __attribute__((aligned(16))) f4_t sg[2][4];  // of a group of 16 tokens: key scale, log2 and inverse of the value scale, hole
+  // of a tile's groups of 16 tokens: key scales (-infinity: a hole), log2 and inverses of the value scales
+  __shared__ __attribute__((aligned(16))) float sg[2][3][4];
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t n = lane & 31u, hl = lane >> 5;
@@ -82,16 +89,15 @@ __global__ __launch_bounds__(64 * W)
     return;
   }
   const int32_t* const table = a.b.table + (size_t)sq * a.b.width;
-  // lane j of every wave keeps the block of group j % 4
-  auto locate = [&](uint32_t tt) -> int32_t {
-    const uint32_t e = (tt * 64u + (lane & 3u) * 16u) >> bsh;
-    int32_t ph = (int32_t)e < seen ? table[e] : -1;
-    if ((uint32_t)ph >= a.c.blocks) ph = -1;
-    return ph;
-  };
+  // Lane j of every wave keeps the block of group j % 4, as the table has it: what has just been asked for is not
+  // looked at, since loads come back in order and to look at the last one is to wait for all.
+  auto entry = [&](uint32_t tt) { return (int32_t)((tt * 64u + (lane & 3u) * 16u) >> bsh); };
+  auto locate = [&](uint32_t tt) -> int32_t { return table[min(entry(tt), seen - 1)]; };
   u4_t kc[CN], vc[CN];
-  f4_t gd;
-  auto load_codes = [&](uint32_t tt, int32_t ph) {
+  float2 gs;    // of the lane's group: the scales
+  bool hole;
+  auto load_codes = [&](uint32_t tt, int32_t raw) {
+    const int32_t ph = entry(tt) < seen && (uint32_t)raw < a.c.blocks ? raw : -1;
 #pragma unroll
     for (int i = 0; i < CN; ++i) {
       const uint32_t c = min(tid + i * 64 * W, kChunks - 1u);
@@ -103,9 +109,8 @@ __global__ __launch_bounds__(64 * W)
       vc[i] = *reinterpret_cast<const u4_t*>(a.c.v + ((cell_v * D + (c >> 2)) << bsh) + slot_v);
     }
     if (tid < 4) {
-      const float2 x = *reinterpret_cast<const float2*>(a.c.scale + ((size_t)max(ph, 0) * a.c.kvh + h) * 2);
-      const float y = ph >= 0 ? fmaxf(x.y, kLeastScale) : 1.f;
-      gd = f4_t{ph >= 0 ? x.x : 0.f, __builtin_amdgcn_logf(y), 1.f / y, ph >= 0 ? 0.f : 1.f};
+      gs = *reinterpret_cast<const float2*>(a.c.scale + ((size_t)max(ph, 0) * a.c.kvh + h) * 2);
+      hole = ph < 0;
     }
   };
   auto store_codes = [&](uint32_t buf) {
@@ -123,14 +128,19 @@ __global__ __launch_bounds__(64 * W)
         vo[1] = u4_t{v1.x, v1.y, v3.x, v3.y};
       }
     }
-    if (tid < 4) sg[buf][tid] = gd;
+    if (tid < 4) {
+      const float y = hole ? 1.f : fmaxf(gs.y, kLeastScale);
+      sg[buf][0][tid] = hole ? -__builtin_inff() : gs.x;
+      sg[buf][1][tid] = __builtin_amdgcn_logf(y);
+      sg[buf][2][tid] = 1.f / y;
+    }
   };
 
-  int32_t ph = -1;
+  int32_t ph = -1;  // of the tile after the one in the registers
   if (t_begin < t_end) {
     ph = locate(t_begin);
     load_codes(t_begin, ph);
-    ph = locate(t_begin + 1);
+    ph = locate(min(t_begin + 1, t_end - 1u));
   }
 
   // The wave's queries: dimensions 16 c + 8 (lane / 32) .., as f16 with a power of two taken out.
@@ -188,15 +198,22 @@ __global__ __launch_bounds__(64 * W)
 
   if (t_begin < t_end) {
     store_codes(0);
-    if (t_begin + 1 < t_end) {
-      load_codes(t_begin + 1, ph);
-      ph = locate(t_begin + 2);
-    }
+    load_codes(min(t_begin + 1, t_end - 1u), ph);
+    ph = locate(min(t_begin + 2, t_end - 1u));
   }
+  // Of the two waves that share a SIMD one goes first, so that its softmax meets the other's products (of eight waves; 1
+  // to 4 %).
+  if (wave & 4u) __builtin_amdgcn_s_setprio(1);
+  auto stage = [&](uint32_t tt) {
+    store_codes((tt - t_begin + 1) & 1u);  // behind the last tile: the last one again, which nobody reads
+    load_codes(min(tt + 2, t_end - 1u), ph);
+    ph = locate(min(tt + 3, t_end - 1u));
+  };
   for (uint32_t tt = t_begin; tt < t_end; ++tt) {
     const uint32_t buf = (tt - t_begin) & 1u;
     const int32_t t0 = (int32_t)(tt * 64u);
     __syncthreads();
+    if constexpr (kAhead) stage(tt);
     if (t0 <= p_most) {
       f16_t sc[2];
 #pragma unroll
@@ -210,20 +227,19 @@ __global__ __launch_bounds__(64 * W)
           const h8_t kf = *reinterpret_cast<const h8_t*>(sk[buf] + (u * 32u + n) * KST + c * 32 + hl * 16);
           sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[c], sc[u], 0, 0, 0);
         }
-      f4_t grp[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) grp[j] = sg[buf][j];
-      const bool hole = grp[0].w + grp[1].w + grp[2].w + grp[3].w != 0.f;
-      const bool mask = __builtin_amdgcn_readfirstlane((int)hole) || t0 + 63 > p_least;
+      const f4_t gk = *reinterpret_cast<const f4_t*>(sg[buf][0]), gl = *reinterpret_cast<const f4_t*>(sg[buf][1]),
+                 gi = *reinterpret_cast<const f4_t*>(sg[buf][2]);
+      const bool holes = fminf(fminf(gk.x, gk.y), fminf(gk.z, gk.w)) == -__builtin_inff();
+      const bool mask = __builtin_amdgcn_readfirstlane((int)holes) || t0 + 63 > p_least;
       h8_t pf[4];
       float kq[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) kq[j] = fmaxf(grp[j].x * qscale, kLeastFactor);
+      for (int j = 0; j < 4; ++j) kq[j] = fmaxf(gk[j] * qscale, kLeastFactor);
       if (mask) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           // tokens 8 x + y (y < 4) of this lane's in group j are seen up to this
-          const int32_t m = grp[j].w != 0.f ? -1 : pos - (t0 + 16 * j + 4 * (int)hl);
+          const int32_t m = gk[j] == -__builtin_inff() ? -1 : pos - (t0 + 16 * j + 4 * (int)hl);
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             if (8 * (i >> 2) + (i & 3) > m) sc[j >> 1][8 * (j & 1) + i] = -__builtin_inff();
@@ -235,7 +251,7 @@ __global__ __launch_bounds__(64 * W)
         float m = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < 8; ++i) m = fmaxf(m, sc[j >> 1][8 * (j & 1) + i]);
-        big = fmaxf(big, __builtin_fmaf(m, kq[j], grp[j].y));
+        big = fmaxf(big, __builtin_fmaf(m, kq[j], gl[j]));
       }
       if (__any(big > R + (kLift + kSlack))) {
         const float row_big = half_max(big);
@@ -251,7 +267,7 @@ __global__ __launch_bounds__(64 * W)
       float part = 0.f;  // at most 2^120: 32 tokens of the least scale
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float c = grp[j].y - R;
+        const float c = gl[j] - R;
         float add = 0.f, p[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -260,7 +276,7 @@ __global__ __launch_bounds__(64 * W)
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) pf[j][i] = (_Float16)p[i];
-        part = __builtin_fmaf(add, grp[j].z, part);
+        part = __builtin_fmaf(add, gi[j], part);
       }
       l.add(part * kSumUnit);
 #pragma unroll
@@ -271,13 +287,7 @@ __global__ __launch_bounds__(64 * W)
           acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[j], acc[d], 0, 0, 0);
         }
     }
-    if (tt + 1 < t_end) {
-      store_codes(buf ^ 1u);
-      if (tt + 2 < t_end) {
-        load_codes(tt + 2, ph);
-        ph = locate(tt + 3);
-      }
-    }
+    if constexpr (!kAhead) stage(tt);
   }
 
   const float sum = half_sum(l.x);
