@@ -50,7 +50,11 @@ namespace {
 
 constexpr uint32_t kStepWaves = 4;
 constexpr uint32_t kJoinWaves = 8;      // of k_join
-constexpr uint32_t kJoinFew = 16;       // splits that k_join_few takes
+constexpr uint32_t kJoinFew = 16;       // splits that k_join_few takes, of rows that see their own part
+// Cross attention takes k_join below this many rows for each split: a workgroup a row costs 5.6 ns a row, a lane
+// that walks its splits 0.4 us a split. Measured, whole calls with k_join and k_join_few: 64 rows of 4 splits 17.4 and 17.7
+// us, of 16 22.1 and 27.6; 1024 of 8 19.4 and 17.7, of 16 23.1 and 25.1; 8192 of 24 233 and 223, of 64 308 and 325.
+constexpr uint64_t kJoinRows = 128;
 constexpr uint32_t kJoinThreads = 256;  // of it
 constexpr uint32_t join_rows(uint32_t dim) { return kJoinThreads / (dim / 4); }
 constexpr uint32_t kRowTile = 16;
@@ -82,8 +86,8 @@ constexpr uint64_t kWideUnits = 256, kWideBytes = 256 << 10;
 // The average, because k_step's grid goes by the rows: 63 single tokens beside a prompt's 512, over 8192 each,
 // 128 dimensions (36 rows) take 368 and 528 us, beside 2048 (132 rows) 822 and 580. The lengths are not known here
 // but for the longest: prompts as ragged as 3 to 1270 tokens (12 heads of 96) take 24 and 34 us.
-bool chunk_pays(uint32_t dim, uint64_t heads, uint64_t group, uint64_t tokens, uint64_t seqs, uint64_t longest, bool full) {
-  const uint64_t rows = group * tokens / seqs, own = full ? 0 : tokens / seqs < longest ? tokens / seqs : longest;
+bool chunk_pays(uint32_t dim, uint64_t heads, uint64_t group, uint64_t tokens, uint64_t seqs, uint64_t longest) {
+  const uint64_t rows = group * tokens / seqs, own = tokens / seqs < longest ? tokens / seqs : longest;
   if (rows <= (dim == 192 ? 255 : 64)) return false;
   const uint64_t row_tiles = heads / group * seqs * ((rows + kRowTile - 1) / kRowTile), seen = longest - own / 2;
   const uint64_t chain = (longest + 63) / 64 < 12 ? (longest + 63) / 64 : 12;
@@ -569,17 +573,91 @@ struct Plan {
   uint32_t tiles, slots, splits, per;
   bool wide, chunk;
   int waves;  // of a workgroup of k_chunk
+  bool join;  // k_join, not k_join_few
   size_t work;
 };
+// Cross attention's plan: the kernel, the waves of a workgroup and the splits with the least expected time. Its rows see
+// all tokens, so that a workgroup's work is known but for the lengths. A workgroup takes `per` tiles of 64 tokens (32 at
+// 256 dimensions) for 16 rows in k_step, whose waves share them out, and for 32 rows a wave in k_chunk; the fullest CU
+// has `load` of them. Expected, in us: what begins and ends a call, the fourth root of the sum of the fourth powers of a wave's chain of tiles, a
+// CU's tiles over its four SIMDs (with `start` for each wave) and the codes' bytes, and the join. Fitted to 4,500
+// random shapes (64 to 256 dimensions, 4 to 20 kv heads of 1 to 16, 1 to 64 sequences, 1 to 1500 rows, 20 to 60,000 tokens) with up to 30 plans
+// each: the chosen plans take 1.5 % more than the best ones (41 % at most), those of the rules for rows that see their own
+// part 9.0 % more. 48 sequences of 1500 tokens, one row, 16 heads of 64: 27 us in one split of four waves, 31 in two; 6 x 448
+// rows over 1500 tokens, 20 heads of 64: 46 us in one split of k_chunk, 54 in two.
+struct Rates {
+  double begin;
+  double chain[5], tile[2][5];  // of each dimension; tile: of four waves, of eight
+  double start[2], mb;          // mb: megabytes in a microsecond
+};
+constexpr Rates kStepRates{5.5, {1.0, 1.2, 1.4, 1.7, 1.4}, {{0.79, 1.0, 1.4, 1.7, 1.7}, {0.78, 0.98, 1.3, 1.6, 1.7}}, {1.4, 1.8}, 6.4};
+constexpr Rates kChunkRates{8.6, {1.0, 1.4, 1.4, 0.0, 0.0}, {{0.62, 0.91, 1.0, 2.3, 3.1}, {0.54, 0.64, 0.72, 0.0, 0.0}}, {2.0, 3.1}, 99.0};
+constexpr double kJoinMb = 2.4, kJoinTime = 2.6, kJoinFewTime = 2.0, kJoinFewSplit = 0.19;
+constexpr uint32_t kCrossSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128};
+constexpr uint64_t kCrossStepRows = 1200, kCrossUnits = 4096;
+
+bool joins_rows(uint64_t rows, uint64_t splits) { return rows < kJoinRows * splits; }
+
+void plan_cross(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, Plan& p) {
+  const uint64_t group = heads / c->kv_heads, rows = group * b->tokens / b->seqs, out_rows = (uint64_t)b->tokens * heads;
+  const uint64_t longest = (uint64_t)most_blocks(c, b) * c->block_tokens;
+  const uint32_t dim = c->dim == 64 ? 0 : c->dim == 96 ? 1 : c->dim == 128 ? 2 : c->dim == 192 ? 3 : 4;
+  const double bytes = 2e-6 * c->dim * c->kv_heads * (double)b->seqs * (double)longest;
+  double least = INFINITY;
+  for (int chunk = 0; chunk < 2; ++chunk) {
+    if (chunk ? rows <= kRowTile : rows > kCrossStepRows) continue;
+    const Rates& r = chunk ? kChunkRates : kStepRates;
+    const uint64_t tokens = chunk ? 64 : step_tile(c->dim), all = (longest + tokens - 1) / tokens;
+    for (int wide = 0; wide < (chunk && c->dim > 128 ? 1 : 2); ++wide) {
+      const int waves = wide ? 8 : 4;
+      const uint32_t row_tile = chunk ? 32u * waves : kRowTile;
+      uint32_t tiles = (uint32_t)((group * b->max_tokens + row_tile - 1) / row_tile);
+      const uint64_t slots = tile_slots(b, group, row_tile, tiles), units = slots * c->kv_heads;
+      uint64_t before = 0;  // the splits looked at last
+      for (const uint32_t want : kCrossSplits) {
+        const uint64_t per = (all + want - 1) / want, splits = (all + per - 1) / per;
+        if (want > 1 && (per < (chunk ? 4u : (uint32_t)waves) || units * splits > kCrossUnits)) break;
+        if (splits == before) continue;
+        before = splits;
+        const double load = (double)((units * splits + 255) / 256);
+        const double chain = r.chain[dim] * (double)(chunk ? per : (per + waves - 1) / waves);
+        const double work = r.tile[wide][dim] * ((double)per * (chunk ? waves : 1) + r.start[wide] * waves) * load / 4;
+        const double read = bytes / r.mb, c2 = chain * chain, w2 = work * work, r2 = read * read;
+        double time = r.begin + std::sqrt(std::sqrt(c2 * c2 + w2 * w2 + r2 * r2));
+        const bool by_row = joins_rows(out_rows, splits);
+        if (splits > 1)
+          time += (by_row ? kJoinTime : kJoinFewTime + kJoinFewSplit * (double)splits) +
+                  4e-6 / kJoinMb * (double)out_rows * (c->dim + 2) * (double)splits;
+        if (time < least) {
+          least = time;
+          p.chunk = chunk;
+          p.wide = !chunk && wide;
+          p.waves = waves;
+          p.tiles = tiles;
+          p.slots = (uint32_t)slots;
+          p.units = units;
+          p.per = (uint32_t)per;
+          p.splits = (uint32_t)splits;
+          p.join = by_row;
+        }
+      }
+    }
+  }
+  if (p.splits > 1) p.work = (size_t)out_rows * p.splits * (c->dim + 2) * 4;
+}
+
 enum Kind { kCausal, kFull, kList };
 Plan plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, Kind kind, uint32_t count) {
   const bool list = kind == kList;
   Plan p{};
   if (b->tokens == 0) return p;
+  if (kind == kFull) {
+    plan_cross(c, b, heads, p);
+    return p;
+  }
   const uint64_t group = heads / c->kv_heads;
   const uint64_t rows = list ? group : group * b->max_tokens;
-  p.chunk = !list && chunk_pays(c->dim, heads, group, b->tokens, b->seqs, (uint64_t)most_blocks(c, b) * c->block_tokens,
-                               kind == kFull);
+  p.chunk = !list && chunk_pays(c->dim, heads, group, b->tokens, b->seqs, (uint64_t)most_blocks(c, b) * c->block_tokens);
   // by the rows that there are: sequences may have fewer than max_tokens
   const uint64_t big = 32 * kChunkWide;
   p.waves = c->dim <= 128 && (group * b->tokens + big - 1) / big * c->kv_heads >= kChunkUnits ? kChunkWide : kChunkSmall;
@@ -604,6 +682,7 @@ Plan plan(const DanceKvCache* c, const DanceKvBatch* b, uint32_t heads, Kind kin
   per = per < least ? least : (per + round - 1) / round * round;
   p.per = (uint32_t)(per < all ? per : all);
   p.splits = (uint32_t)((all + p.per - 1) / p.per);
+  p.join = p.splits > kJoinFew;
   if (p.splits > 1) p.work = (size_t)b->tokens * heads * p.splits * (c->dim + 2) * 4;
   return p;
 }
@@ -634,8 +713,8 @@ int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, c
   }
   // Rows are counted in 31 bits, a launch's threads in 32; the joins' grids count where there is a join.
   const uint64_t grid = p.units * p.splits, rows = (uint64_t)batch->tokens * q->heads;
-  const uint64_t join = p.splits > kJoinFew ? rows * 64 * kJoinWaves
-                        : p.splits > 1      ? (rows / join_rows(cache->dim) + 1) * kJoinThreads
+  const uint64_t join = p.splits > 1 && p.join ? rows * 64 * kJoinWaves
+                        : p.splits > 1         ? (rows / join_rows(cache->dim) + 1) * kJoinThreads
                                             : 0;
   if (grid * 64 * 8 > 0xFFFFFFFFull || rows > 0x7FFFFFFFull || join > 0xFFFFFFFFull) {
     std::fprintf(stderr, "[%s] batch is too large for one launch\n", who);
@@ -672,7 +751,7 @@ int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, c
       vec ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
     else
       vec ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
-    if (p.splits > kJoinFew)
+    if (p.splits > 1 && p.join)
       hipLaunchKernelGGL((k_join<D, BF>), dim3((uint32_t)rows), dim3(64 * kJoinWaves), 0, st, a.part, p.splits, rows,
                          a.out, lse);
     else if (p.splits > 1)

@@ -537,8 +537,8 @@ const char* check_layers(const DanceKvCache* c, uint32_t n) {
     const DanceKvBatch one{nullptr, nullptr, nullptr, 1, 0, 1, 1, 0};
     if (const char* why = check_shapes(c + i, &one)) return why;
     if (!c[i].k || !c[i].v || !c[i].scale || !c[i].bound) return "null cache pointer";
-    if (!aligned(c[i].k, 16) || !aligned(c[i].v, 16) || !aligned(c[i].scale, 16) || !aligned(c[i].bound, 16))
-      return "the cache's arrays must be aligned to 16 bytes";
+    if (!aligned(c[i].k, 16) || !aligned(c[i].v, 16) || !aligned(c[i].scale, 8) || !aligned(c[i].bound, 16))
+      return "the caches' arrays must be aligned to 16 bytes, their scales to 8";
     if (c[i].kv_heads != c->kv_heads || c[i].dim != c->dim || c[i].block_tokens != c->block_tokens || c[i].blocks != c->blocks)
       return "the caches must have one kv_heads, dim, block_tokens and number of blocks";
   }

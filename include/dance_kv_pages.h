@@ -60,7 +60,8 @@ int dance_kv_release(const DanceKvPages *pages, int32_t *table, int32_t *lengths
 /* Copies block src[i] of from[c] to block dst[i] of to[c], for each of `caches`
  * caches (a model's layers) and `pairs` pairs. A pair with either outside its
  * cache is left out. All caches have one kv_heads, dim and block_tokens, all of `from` one number of blocks and all
- * of `to` one. `to` may be `from`; then no block may be both a source and a
+ * of `to` one; scales need no more than 8 bytes' alignment here (a layer's part of one array of many layers). `to` may be
+ * `from`; then no block may be both a source and a
  * destination. No block may be a destination twice. */
 int dance_kv_copy(const DanceKvCache *from, const DanceKvCache *to, uint32_t caches, const int32_t *src, const int32_t *dst,
                   uint32_t pairs, void *stream);

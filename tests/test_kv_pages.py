@@ -265,6 +265,19 @@ def test_copy(layers, heads, dim, bs, pairs, other):
 
 
 @pytest.mark.gpu
+def test_copy_of_layers_in_one_array():
+    """Layers whose scales begin at any multiple of 8 bytes."""
+    rng, shape = np.random.default_rng(11), (4, 5, 3)  # layers, blocks, heads
+    k, v, b = (dev(rng.integers(-128, 128, shape + x, dtype=np.int8)) for x in ((16, 64), (64, 16), (2, 64)))
+    s = dev(np.float32(rng.random(shape + (2,))))
+    want = [x.clone() for x in (k, v, s, b)]
+    for x in want:
+        x[:, 4] = x[:, 1]
+    kv.copy([kv.KVCache(k[i], v[i], s[i], b[i]) for i in range(4)], dev(np.int32([1, -1])), dev(np.int32([4, 0])))
+    assert all(torch.equal(x, y) for x, y in zip((k, v, s, b), want))
+
+
+@pytest.mark.gpu
 def test_copy_and_compact_beyond_32_bit_offsets():
     heads, bs, dim = 8, 128, 256
     blocks = (1 << 32) // (heads * bs * dim) + 40
@@ -655,7 +668,7 @@ def test_entries_refuse_before_any_device_work(capfd):
               (L.dance_kv_reserve, [ok, p, p, 1 << 20, 1 << 12, p, p, p, p, p, 1 << 50, None]),
               (L.dance_kv_release, [ok, None, p, 2, 3, p, p, None]), (L.dance_kv_release, [ok, p, None, 2, 3, p, p, None])]
     c = fake()[0]
-    for change in ({"k": None}, {"scale": p | 8}, {"dim": 100}, {"block_tokens": 8}, {"blocks": 0}, {"kv_heads": 0}):
+    for change in ({"k": None}, {"scale": p | 4}, {"bound": p | 8}, {"dim": 100}, {"block_tokens": 8}, {"blocks": 0}, {"kv_heads": 0}):
         bad = fake(**change)[0]
         calls += [(L.dance_kv_copy, [bad, c, 1, p, p, 2, None]), (L.dance_kv_copy, [c, bad, 1, p, p, 2, None]),
                   (L.dance_kv_compact, [bad, c, p, p, 2, 3, p, 2, 5, p, p, 3, None]),
