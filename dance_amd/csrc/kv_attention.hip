@@ -50,11 +50,13 @@ namespace {
 
 constexpr uint32_t kStepWaves = 4;
 constexpr uint32_t kJoinWaves = 8;      // of k_join
+constexpr uint32_t kJoinCrossWaves = 4;  // of k_join_cross
 constexpr uint32_t kJoinFew = 16;       // splits that k_join_few takes, of rows that see their own part
 // Cross attention takes k_join below this many rows for each split: a workgroup a row costs 5.6 ns a row, a lane
 // that walks its splits 0.4 us a split. Measured, whole calls with k_join and k_join_few: 64 rows of 4 splits 17.4 and 17.7
 // us, of 16 22.1 and 27.6; 1024 of 8 19.4 and 17.7, of 16 23.1 and 25.1; 8192 of 24 233 and 223, of 64 308 and 325.
 constexpr uint64_t kJoinRows = 128;
+constexpr uint64_t kJoinCrossRows = 256;  // from here on k_join_cross
 constexpr uint32_t kJoinThreads = 256;  // of it
 constexpr uint32_t join_rows(uint32_t dim) { return kJoinThreads / (dim / 4); }
 constexpr uint32_t kRowTile = 16;
@@ -166,8 +168,7 @@ __device__ __forceinline__ u2_t quotients(f4_t o, float l) {
 constexpr int step_tile(int d) { return d <= 192 ? 64 : 32; }
 
 template <int D, bool BF, bool LIST, bool VEC, uint32_t W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_step(
-    StepArgs a) {
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) void k_step(StepArgs a) {
   constexpr int KS = D / 32;  // inner steps of the first product
   constexpr int DT = D / 16;  // row tiles of the second
   constexpr int KW = D / 16;  // words of a key row that a lane holds
@@ -514,18 +515,17 @@ __global__ __launch_bounds__(kJoinThreads) void k_join_few(const float* __restri
   if (lse && d == 0) lse[row] = lse_of(m, total);
 }
 
-// Joins a row's many splits, one workgroup per row: the weights of up to 64
+// Joins a row's many splits, W waves for the row: the weights of up to 64
 // splits at a time in the lanes of every wave, the sums of the splits that have
 // any shared out over the waves. (One wave per row that walked its splits took
-// 155 us for 32 rows of 256 splits; so 11.)
-template <int D, bool BF>
-__global__ __launch_bounds__(64 * kJoinWaves) void k_join(const float* __restrict__ part, uint32_t splits, uint64_t rows,
-                                                          uint16_t* __restrict__ out, float* __restrict__ lse) {
+// 155 us for 32 rows of 256 splits; eight so 11.)
+template <int D, bool BF, uint32_t W>
+__device__ __forceinline__ void join_row(const float* __restrict__ part, uint32_t splits, uint64_t rows, uint64_t row,
+                                         uint16_t* __restrict__ out, float* __restrict__ lse) {
   constexpr uint32_t L = D / 4;  // lanes that a row of sums takes
   constexpr uint32_t P = 64 / L > 0 ? 64 / L : 1;
-  __shared__ f4_t sums[kJoinWaves][64];
+  __shared__ f4_t sums[W][64];
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint64_t row = blockIdx.x;
   const float* const ml = part + rows * splits * D + row * splits * 2;
   const float* const po = part + row * splits * D;
   float m = -FLT_MAX;
@@ -540,16 +540,18 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_join(const float* __restric
     const float f = l != 0.f ? exp2f(ml[2 * i] - m) : 0.f;
     total += f * l;
     const uint32_t n = min(64u, splits - i0);
+#pragma unroll 1
+    for (uint32_t k0 = wave * P; k0 < n; k0 += 8 * W * P)
 #pragma unroll
-    for (uint32_t k = wave * P; k < 64; k += kJoinWaves * P) {
-      if (k >= n) continue;
-      const uint32_t at = k + lane / L;
-      const float other = __shfl(f, (int)min(at, 63u)), w = at < 64u && lane < P * L ? other : 0.f;
-      // without sums: the first split's line again, as above
-      const f4_t x = *reinterpret_cast<const f4_t*>(po + (size_t)(w != 0.f ? i0 + at : 0u) * D + lane % L * 4);
+      for (uint32_t k = k0; k < k0 + 8 * W * P; k += W * P) {
+        if (k >= n) continue;
+        const uint32_t at = k + lane / L;
+        const float other = __shfl(f, (int)min(at, 63u)), w = at < 64u && lane < P * L ? other : 0.f;
+        // without sums: the first split's line again, as above
+        const f4_t x = *reinterpret_cast<const f4_t*>(po + (size_t)(w != 0.f ? i0 + at : 0u) * D + lane % L * 4);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) o[c] += w != 0.f ? w * x[c] : 0.f;
-    }
+        for (int c = 0; c < 4; ++c) o[c] += w != 0.f ? w * x[c] : 0.f;
+      }
   }
 #pragma unroll
   for (int x = 1; x < 64; x <<= 1) total += __shfl_xor(total, x);
@@ -558,7 +560,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_join(const float* __restric
   if (wave == 0 && lane < L) {
     f4_t y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (uint32_t w = 0; w < kJoinWaves; ++w)
+    for (uint32_t w = 0; w < W; ++w)
 #pragma unroll
       for (uint32_t p = 0; p < P; ++p)
 #pragma unroll
@@ -566,6 +568,18 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_join(const float* __restric
     *reinterpret_cast<u2_t*>(out + row * D + lane * 4) = quotients<BF>(y, total);
     if (lse && lane == 0) lse[row] = lse_of(m, total);
   }
+}
+template <int D, bool BF>
+__global__ __launch_bounds__(64 * kJoinWaves) void k_join(const float* __restrict__ part, uint32_t splits, uint64_t rows,
+                                                          uint16_t* __restrict__ out, float* __restrict__ lse) {
+  join_row<D, BF, kJoinWaves>(part, splits, rows, blockIdx.x, out, lse);
+}
+// Of cross attention, where there may be many rows too: 2048 rows of 32 splits 74 us in all with eight waves a row, 71 with
+// four; 64 rows of 128 splits 32 and 34.
+template <int D, bool BF>
+__global__ __launch_bounds__(64 * kJoinCrossWaves) void k_join_cross(const float* __restrict__ part, uint32_t splits, uint64_t rows,
+                                                                     uint16_t* __restrict__ out, float* __restrict__ lse) {
+  join_row<D, BF, kJoinCrossWaves>(part, splits, rows, blockIdx.x, out, lse);
 }
 
 struct Plan {
@@ -580,19 +594,19 @@ struct Plan {
 // all tokens, so that a workgroup's work is known but for the lengths. A workgroup takes `per` tiles of 64 tokens (32 at
 // 256 dimensions) for 16 rows in k_step, whose waves share them out, and for 32 rows a wave in k_chunk; the fullest CU
 // has `load` of them. Expected, in us: what begins and ends a call, the fourth root of the sum of the fourth powers of a wave's chain of tiles, a
-// CU's tiles over its four SIMDs (with `start` for each wave) and the codes' bytes, and the join. Fitted to 4,500
+// CU's tiles over its four SIMDs (with `start` for each wave) and the codes' bytes, and the join. Fitted to 5,000
 // random shapes (64 to 256 dimensions, 4 to 20 kv heads of 1 to 16, 1 to 64 sequences, 1 to 1500 rows, 20 to 60,000 tokens) with up to 30 plans
-// each: the chosen plans take 1.5 % more than the best ones (41 % at most), those of the rules for rows that see their own
-// part 9.0 % more. 48 sequences of 1500 tokens, one row, 16 heads of 64: 27 us in one split of four waves, 31 in two; 6 x 448
+// each: the chosen plans take 1.4 % more than the best ones (48 % at most), those of the rules for rows that see their own
+// part 9 % more. 48 sequences of 1500 tokens, one row, 16 heads of 64: 27 us in one split of four waves, 31 in two; 6 x 448
 // rows over 1500 tokens, 20 heads of 64: 46 us in one split of k_chunk, 54 in two.
 struct Rates {
   double begin;
   double chain[5], tile[2][5];  // of each dimension; tile: of four waves, of eight
   double start[2], mb;          // mb: megabytes in a microsecond
 };
-constexpr Rates kStepRates{5.5, {1.0, 1.2, 1.4, 1.7, 1.4}, {{0.79, 1.0, 1.4, 1.7, 1.7}, {0.78, 0.98, 1.3, 1.6, 1.7}}, {1.4, 1.8}, 6.4};
-constexpr Rates kChunkRates{8.6, {1.0, 1.4, 1.4, 0.0, 0.0}, {{0.62, 0.91, 1.0, 2.3, 3.1}, {0.54, 0.64, 0.72, 0.0, 0.0}}, {2.0, 3.1}, 99.0};
-constexpr double kJoinMb = 2.4, kJoinTime = 2.6, kJoinFewTime = 2.0, kJoinFewSplit = 0.19;
+constexpr Rates kStepRates{5.9, {1.1, 1.2, 1.4, 1.6, 1.2}, {{0.67, 0.93, 1.4, 1.8, 1.8}, {0.61, 0.97, 1.3, 1.6, 1.7}}, {1.3, 1.7}, 6.4};
+constexpr Rates kChunkRates{8.7, {1.0, 1.4, 1.4, 0.0, 0.0}, {{0.59, 0.92, 1.0, 2.3, 3.1}, {0.52, 0.65, 0.73, 0.0, 0.0}}, {2.0, 3.2}, 120.0};
+constexpr double kJoinMb = 2.6, kJoinTime = 2.5, kJoinFewTime = 2.0, kJoinFewSplit = 0.24;
 constexpr uint32_t kCrossSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128};
 constexpr uint64_t kCrossStepRows = 1200, kCrossUnits = 4096;
 
@@ -751,7 +765,10 @@ int run(const char* who, const DanceKvCache* cache, const DanceKvBatch* batch, c
       vec ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
     else
       vec ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
-    if (p.splits > 1 && p.join)
+    if (p.splits > 1 && p.join && kind == kFull && rows >= kJoinCrossRows)
+      hipLaunchKernelGGL((k_join_cross<D, BF>), dim3((uint32_t)rows), dim3(64 * kJoinCrossWaves), 0, st, a.part, p.splits, rows,
+                         a.out, lse);
+    else if (p.splits > 1 && p.join)
       hipLaunchKernelGGL((k_join<D, BF>), dim3((uint32_t)rows), dim3(64 * kJoinWaves), 0, st, a.part, p.splits, rows,
                          a.out, lse);
     else if (p.splits > 1)

@@ -122,7 +122,7 @@ def test_plans_reach_every_kernel():
     if not ran:
         pytest.skip("torch's profiler does not name the kernels here")
     kinds = {k.split("<")[0] + ("-" + k[:-1].split(", ")[-1] if "join" not in k else "") for k in ran}
-    assert kinds == {"k_step-4", "k_step-8", "k_chunk-4", "k_chunk-8", "k_join", "k_join_few"}
+    assert kinds == {"k_step-4", "k_step-8", "k_chunk-4", "k_chunk-8", "k_join", "k_join_cross", "k_join_few"}
 
 
 def check_cross_large(cache, got, lse, q, table, lens, off, scale):
