@@ -41,16 +41,18 @@ __device__ __forceinline__ uint32_t block_sum(uint32_t x, uint32_t* lds) {
 
 // ---------------------------------------------------------------- fork
 
-// Workgroups of old rows change the counts, by a row's children less one: where a
-// row goes on as one, in whatever slot, nothing is to be counted. Those of new
-// rows copy them, behind the others, whose atomics take longer.
+constexpr uint32_t kTogether = 8;  // old rows that a workgroup looks at
+
+// Workgroups of old rows change the counts, by a row's children less one. A thread takes a place of several
+// rows: rows that lie together, as beams do, mostly share their first blocks, and what one of them loses there another
+// gains (128 users of 4 beams, 500 to 60,000 tokens in blocks of 32: 10.8 us with an atomic for each entry, 7.0
+// so). Workgroups of new rows copy them.
 __global__ __launch_bounds__(kThreads) void k_fork(Pages p, Table t, const int32_t* __restrict__ parents, uint32_t fresh,
-                                                   uint32_t runs, int32_t* __restrict__ table, int32_t* __restrict__ lengths) {
-  __shared__ uint32_t lds[kWaves];
-  const uint32_t run = blockIdx.x % runs, row = blockIdx.x / runs;
-  const uint32_t e0 = run * kRun + threadIdx.x;
-  if (row >= t.seqs) {
-    const uint32_t to = row - t.seqs;
+                                                   uint32_t runs, uint32_t parts, uint32_t olds, int32_t* __restrict__ table,
+                                                   int32_t* __restrict__ lengths) {
+  __shared__ int32_t more[kTogether];
+  if (blockIdx.x >= olds) {
+    const uint32_t run = (blockIdx.x - olds) % runs, to = (blockIdx.x - olds) / runs, e0 = run * kRun + threadIdx.x;
     const int32_t from = parents[to];
     const bool ok = (uint32_t)from < t.seqs;
     const int32_t* const src = t.table + (size_t)(ok ? from : 0) * t.width;
@@ -64,17 +66,32 @@ __global__ __launch_bounds__(kThreads) void k_fork(Pages p, Table t, const int32
     if (run == 0 && threadIdx.x == 0) lengths[to] = ok ? t.lengths[from] : 0;
     return;
   }
-  const int32_t* const src = t.table + (size_t)row * t.width;
-  int32_t x[kEntries];
+  const uint32_t row0 = blockIdx.x / parts * kTogether, place = blockIdx.x % parts * kThreads + threadIdx.x;
+  const uint32_t rows = min(kTogether, t.seqs - row0);
+  int32_t x[kTogether];
 #pragma unroll
-  for (uint32_t i = 0; i < kEntries; ++i) x[i] = src[min(e0 + i * kThreads, t.width - 1u)];
-  uint32_t mine = 0;
-  for (uint32_t i = threadIdx.x; i < fresh; i += kThreads) mine += (uint32_t)parents[i] == row ? 1u : 0u;
-  const int32_t more = (int32_t)block_sum(mine, lds) - 1;
-  if (more == 0) return;
+  for (uint32_t r = 0; r < kTogether; ++r)
+    x[r] = t.table[(size_t)(row0 + min(r, rows - 1u)) * t.width + min(place, t.width - 1u)];
+  if (threadIdx.x < kTogether) more[threadIdx.x] = -1;
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < fresh; i += kThreads) {
+    const uint32_t r = (uint32_t)parents[i] - row0;
+    if (r < rows) atomicAdd(more + r, 1);
+  }
+  __syncthreads();
+  if (place >= t.width) return;
+  int32_t block = x[0], by = 0;
 #pragma unroll
-  for (uint32_t i = 0; i < kEntries; ++i)
-    if (e0 + i * kThreads < t.width && (uint32_t)x[i] < p.blocks) atomicAdd(p.refs + x[i], more);
+  for (uint32_t r = 0; r < kTogether; ++r) {
+    if (r >= rows) break;
+    if (x[r] != block) {
+      if (by != 0 && (uint32_t)block < p.blocks) atomicAdd(p.refs + block, by);
+      block = x[r];
+      by = 0;
+    }
+    by += more[r];
+  }
+  if (by != 0 && (uint32_t)block < p.blocks) atomicAdd(p.refs + block, by);
 }
 
 // ------------------------------------------------------------- reserve
@@ -113,11 +130,18 @@ struct Free {
   uint64_t word;
   uint32_t count;
 };
-__device__ __forceinline__ Free free_of(const Pages& p, uint32_t at, uint32_t lane) {
+struct Refs {
   int32_t r[kWords];
-  const uint32_t b0 = at * kFree + lane;
+};
+__device__ __forceinline__ Refs refs_of(const Pages& p, uint32_t at, uint32_t lane) {
+  Refs x;
 #pragma unroll
-  for (uint32_t i = 0; i < kWords; ++i) r[i] = p.refs[min(b0 + i * 64, p.blocks - 1u)];
+  for (uint32_t i = 0; i < kWords; ++i) x.r[i] = p.refs[min(at * kFree + lane + i * 64, p.blocks - 1u)];
+  return x;
+}
+__device__ __forceinline__ Free free_of(const Pages& p, const Refs& x, uint32_t at, uint32_t lane) {
+  const int32_t* const r = x.r;
+  const uint32_t b0 = at * kFree + lane;
   Free f{0, 0};
 #pragma unroll
   for (uint32_t i = 0; i < kWords; ++i) {
@@ -145,7 +169,7 @@ __global__ __launch_bounds__(kThreads) void k_needs(Pages p, Table t, const int3
   if (blockIdx.x >= t.seqs) {
     const uint32_t at = (blockIdx.x - t.seqs) * kWaves + wave;
     if (at >= n.counts) return;
-    const Free f = free_of(p, at, lane);
+    const Free f = free_of(p, refs_of(p, at, lane), at, lane);
     if (lane < kWords) n.free[(size_t)at * kWords + lane] = f.word;
     if (lane == 0) n.count[at] = f.count;
     return;
@@ -315,6 +339,7 @@ __global__ __launch_bounds__(64 * kSmall) void k_reserve(Pages p, Table t, const
   __shared__ uint64_t free[kSmall][kWords], fresh[64][kSmallWords];
   __shared__ uint32_t count[kSmall], need[64];
   const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const Refs run = refs_of(p, min(wave, counts - 1u), lane);  // asked for before the way to the sequences' blocks
   // Lane b of every wave knows sequence b.
   Growth g{};
   int32_t block = -1, refs = 0;
@@ -324,7 +349,7 @@ __global__ __launch_bounds__(64 * kSmall) void k_reserve(Pages p, Table t, const
     if ((uint32_t)block < p.blocks) refs = p.refs[block];
   }
   if (wave < counts) {
-    const Free f = free_of(p, wave, lane);
+    const Free f = free_of(p, run, wave, lane);
     if (lane < kWords) free[wave][lane] = f.word;
     if (lane == 0) count[wave] = f.count;
   } else if (lane == 0) {
@@ -348,7 +373,8 @@ __global__ __launch_bounds__(64 * kSmall) void k_reserve(Pages p, Table t, const
     const uint64_t tail = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)copies, (int)b);
     uint32_t sum = 0;
     for (uint32_t w = 0; o.first + w * 64 < o.end; ++w) {
-      const uint64_t mask = fresh_of(p, o, t.table + (size_t)b * t.width, o.first + w * 64, lane) | (w ? 0ull : tail);
+      const bool known = o.partly && o.end - o.first == 1;  // a token more in a block that has some
+      const uint64_t mask = (known ? 0ull : fresh_of(p, o, t.table + (size_t)b * t.width, o.first + w * 64, lane)) | (w ? 0ull : tail);
       sum += (uint32_t)__popcll(mask);
       if (lane == 0) fresh[b][w] = mask;
     }
@@ -560,12 +586,12 @@ int dance_kv_fork(const DanceKvPages* pages, const int32_t* table, const int32_t
   if (!why && (new_seqs == 0 || new_seqs > 0x7FFFFFFFu)) why = "new_seqs must be positive, below 2^31";
   if (!why && (table == new_table || lengths == new_lengths)) why = "the new arrays must not be the old ones";
   if (why) KV_ERR("dance_kv_fork", "%s", why);
-  const uint32_t runs = runs_of(width);
-  const uint64_t grid = ((uint64_t)seqs + new_seqs) * runs;
+  const uint32_t runs = runs_of(width), parts = (width + kThreads - 1) / kThreads;
+  const uint64_t olds = ((uint64_t)seqs + kTogether - 1) / kTogether * parts, grid = olds + (uint64_t)new_seqs * runs;
   if (too_many(grid)) KV_ERR("dance_kv_fork", "batch is too large for one launch");
   const Table t{const_cast<int32_t*>(table), const_cast<int32_t*>(lengths), seqs, width};
   hipLaunchKernelGGL(k_fork, dim3((uint32_t)grid), dim3(kThreads), 0, static_cast<hipStream_t>(stream), pages_args(pages), t,
-                     parents, new_seqs, runs, new_table, new_lengths);
+                     parents, new_seqs, runs, parts, (uint32_t)olds, new_table, new_lengths);
   return launched("dance_kv_fork");
 }
 

@@ -694,3 +694,18 @@ def test_entries_refuse_before_any_device_work(capfd):
         assert fn.__name__ in capfd.readouterr().err
     assert L.dance_kv_copy(c, c, 1, None, None, 0, None) == 0  # no pairs: nothing to do
     assert L.dance_kv_release(ok, p, p, 2, 3, None, None, None) == 0
+
+
+@pytest.mark.gpu
+def test_example_of_beam_decoding():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "kv_beams.py")
+    spec = importlib.util.spec_from_file_location("kv_beams", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    got = module.run(users=3, beams=4, prompt=1500, steps=20, layers=2, heads=8, kv_heads=2, block_tokens=32, quiet=True)
+    assert len(got) == 20 and all(r["missed"] == 0 and r["owned"] <= r["named"] for r in got)
+    # three roundings to bfloat16 and the weights' to 11 bits, of outputs of about one size: a few 2^-9 of their norm
+    assert all(r["apart"] < 2.0 ** -6 for r in got)
+    assert got[-1]["left"] == sum(-(-((1500 - 331 * u + 21) // 2) // 32) for u in range(3))
