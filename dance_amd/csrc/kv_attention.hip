@@ -49,15 +49,15 @@ namespace kv {
 namespace {
 
 constexpr uint32_t kStepWaves = 4;
-constexpr uint32_t kJoinWaves = 8;      // of k_join
+constexpr uint32_t kJoinWaves = 8;       // of k_join
 constexpr uint32_t kJoinCrossWaves = 4;  // of k_join_cross
-constexpr uint32_t kJoinFew = 16;       // splits that k_join_few takes, of rows that see their own part
+constexpr uint32_t kJoinFew = 16;        // splits that k_join_few takes, of rows that see their own part
 // Cross attention takes k_join below this many rows for each split: a workgroup a row costs 5.6 ns a row, a lane
 // that walks its splits 0.4 us a split. Measured, whole calls with k_join and k_join_few: 64 rows of 4 splits 17.4 and 17.7
 // us, of 16 22.1 and 27.6; 1024 of 8 19.4 and 17.7, of 16 23.1 and 25.1; 8192 of 24 233 and 223, of 64 308 and 325.
 constexpr uint64_t kJoinRows = 128;
 constexpr uint64_t kJoinCrossRows = 256;  // from here on k_join_cross
-constexpr uint32_t kJoinThreads = 256;  // of it
+constexpr uint32_t kJoinThreads = 256;    // of k_join_few
 constexpr uint32_t join_rows(uint32_t dim) { return kJoinThreads / (dim / 4); }
 constexpr uint32_t kRowTile = 16;
 // Waves of a workgroup that takes all of a row tile's tokens. It needs no join (and
@@ -577,8 +577,9 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_join(const float* __restric
 // Of cross attention, where there may be many rows too: 2048 rows of 32 splits 74 us in all with eight waves a row, 71 with
 // four; 64 rows of 128 splits 32 and 34.
 template <int D, bool BF>
-__global__ __launch_bounds__(64 * kJoinCrossWaves) void k_join_cross(const float* __restrict__ part, uint32_t splits, uint64_t rows,
-                                                                     uint16_t* __restrict__ out, float* __restrict__ lse) {
+__global__ __launch_bounds__(64 * kJoinCrossWaves) void k_join_cross(const float* __restrict__ part, uint32_t splits,
+                                                                     uint64_t rows, uint16_t* __restrict__ out,
+                                                                     float* __restrict__ lse) {
   join_row<D, BF, kJoinCrossWaves>(part, splits, rows, blockIdx.x, out, lse);
 }
 
@@ -591,21 +592,23 @@ struct Plan {
   size_t work;
 };
 // Cross attention's plan: the kernel, the waves of a workgroup and the splits with the least expected time. Its rows see
-// all tokens, so that a workgroup's work is known but for the lengths. A workgroup takes `per` tiles of 64 tokens (32 at
-// 256 dimensions) for 16 rows in k_step, whose waves share them out, and for 32 rows a wave in k_chunk; the fullest CU
-// has `load` of them. Expected, in us: what begins and ends a call, the fourth root of the sum of the fourth powers of a wave's chain of tiles, a
-// CU's tiles over its four SIMDs (with `start` for each wave) and the codes' bytes, and the join. Fitted to 5,000
-// random shapes (64 to 256 dimensions, 4 to 20 kv heads of 1 to 16, 1 to 64 sequences, 1 to 1500 rows, 20 to 60,000 tokens) with up to 30 plans
-// each: the chosen plans take 1.4 % more than the best ones (48 % at most), those of the rules for rows that see their own
-// part 9 % more. 48 sequences of 1500 tokens, one row, 16 heads of 64: 27 us in one split of four waves, 31 in two; 6 x 448
-// rows over 1500 tokens, 20 heads of 64: 46 us in one split of k_chunk, 54 in two.
+// all tokens, so that a workgroup's work is known but for the lengths. A workgroup takes `per` tiles of 64 tokens (32
+// at 256 dimensions in k_step) for 16 rows in k_step, whose waves share them out, and for 32 rows a wave in k_chunk; the
+// fullest CU has `load` of them. Expected, in us: what begins and ends a call; the fourth root of the sum of the fourth
+// powers of a wave's chain of tiles, a CU's tiles over its four SIMDs (with `start` more for each wave) and the codes'
+// bytes; and the join. Fitted to 5,000 random shapes (64 to 256 dimensions, 1 to 20 kv heads of 1 to 16, 1 to 64 sequences,
+// 1 to 1500 rows, 20 to 60,000 tokens) with up to 30 plans each: on 800 others the chosen plans take 2.3 % more than the
+// best ones on average, those of the rules for rows that see their own part took 9 % more. 48 sequences of 1500 tokens, one row, 16
+// heads of 64: 27 us in one split, 31 in the two of those rules; 6 x 448 rows over 1500 tokens, 20 heads of 64: 46 and 54.
 struct Rates {
   double begin;
   double chain[5], tile[2][5];  // of each dimension; tile: of four waves, of eight
   double start[2], mb;          // mb: megabytes in a microsecond
 };
-constexpr Rates kStepRates{5.9, {1.1, 1.2, 1.4, 1.6, 1.2}, {{0.67, 0.93, 1.4, 1.8, 1.8}, {0.61, 0.97, 1.3, 1.6, 1.7}}, {1.3, 1.7}, 6.4};
-constexpr Rates kChunkRates{8.7, {1.0, 1.4, 1.4, 0.0, 0.0}, {{0.59, 0.92, 1.0, 2.3, 3.1}, {0.52, 0.65, 0.73, 0.0, 0.0}}, {2.0, 3.2}, 120.0};
+constexpr Rates kStepRates{
+    5.9, {1.1, 1.2, 1.4, 1.6, 1.2}, {{0.67, 0.93, 1.4, 1.8, 1.8}, {0.61, 0.97, 1.3, 1.6, 1.7}}, {1.3, 1.7}, 6.4};
+constexpr Rates kChunkRates{
+    8.7, {1.0, 1.4, 1.4, 0.0, 0.0}, {{0.59, 0.92, 1.0, 2.3, 3.1}, {0.52, 0.65, 0.73, 0.0, 0.0}}, {2.0, 3.2}, 120.0};
 constexpr double kJoinMb = 2.6, kJoinTime = 2.5, kJoinFewTime = 2.0, kJoinFewSplit = 0.24;
 constexpr uint32_t kCrossSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128};
 constexpr uint64_t kCrossStepRows = 1200, kCrossUnits = 4096;

@@ -11,11 +11,11 @@
 // are bytes of different lines: lanes stand for neighbouring tokens, which mostly lie in the same lines, and leave as
 // words of four tokens that four lanes exchange by DPP.
 //
-// Measured: all tokens of 31 sequences of 15,000 to 21,000 copied (96 dimensions), 46 us, 4.9 TB/s, a large copy's rate. Half of 16 sequences of
-// 4,000 to 24,000 (8 heads of 128), other tokens for each head, 97 us: 290 MB that count, 371 that move, since a line of
-// values comes whole; 3.8 TB/s, and the units that form the byte loads' addresses are busy for two thirds of the time. Every
-// fiftieth token of 262,144: 39 us, all of the values' lines (268 MB, 6.9 TB/s). Lines read whole and bytes taken
-// out of LDS: 90 us for half of the tokens, but 61 for all of them and 38 -> 60 at 256 dimensions.
+// Measured: all tokens of 31 sequences of 15,000 to 21,000 copied (96 dimensions), 46 us, 4.9 TB/s, a large copy's
+// rate. Half of 16 sequences of 4,000 to 24,000 (8 heads of 128), other tokens for each head, 96 us: 290 MB that count,
+// 371 that move, since a line of values comes whole; 3.9 TB/s, and the units that form the byte loads' addresses are
+// busy for two thirds of the time. Every fiftieth token of 262,144: 50 us, all of the values' lines (268 MB, 5.4 TB/s).
+// Lines read whole and bytes taken out of LDS: 90 us for half of the tokens, but 61 for all of the 31 sequences.
 //
 // Between powers of two the arithmetic is f16's, two codes an instruction: a code is exact there, and c * ratio +
 // 1536 has the unit 1, so that one fma rounds it as the definition does and leaves the code in the low byte.
@@ -79,8 +79,8 @@ __global__ __launch_bounds__(64 * compact_waves(D, BS)) void k_compact(Compact a
   constexpr uint32_t W = compact_waves(D, BS), T = 64 * W;
   constexpr uint32_t C16 = D / 16, R = T / C16 < BS ? T / C16 : BS;  // keys: pieces of a token, tokens at once
   constexpr uint32_t NP = (BS + R - 1) / R;                         // pieces of a lane
-  constexpr uint32_t G = T / BS, NW = D / 4 / G;                    // values: lanes of a token, words of four dimensions of a lane
-  static_assert(T % BS == 0 && D / 4 % G == 0, "every lane has a token and as many dimensions");
+  constexpr uint32_t G = T / BS, NW = D / 4 / G;                    // values: lanes of a token, fours of dimensions of a lane
+  static_assert(T % BS == 0 && D / 4 % G == 0, "every lane has a token, and as many dimensions as the others");
   __shared__ uint32_t t_cell[BS], t_slot[BS];
   __shared__ float2 t_scale[BS];
   __shared__ float wave_max[W][2];
@@ -194,8 +194,8 @@ __global__ __launch_bounds__(64 * compact_waves(D, BS)) void k_compact(Compact a
   const float inv_k = exp2_int(-ek), inv_v = exp2_int(-ev);
   if (tid == 0) *reinterpret_cast<float2*>(a.to.scale + cell * 2) = float2{exp2_int(ek), exp2_int(ev)};
 
-  // Four codes of scale s, as halves 1536 + code. A code that is not 0 has a ratio of at most 2^6 then, and one
-  // below 2^-8 rounds it to 0.
+  // Four codes of scale s, as halves 1536 + code. A code that is not 0 has a ratio of at most 2^6, since the new scale
+  // holds it; and one below 2^-8 rounds it to 0, as f16's least numbers do.
   auto rounded = [&](u2_t c, float s, float inv) {
     const h2_t unit = {(_Float16)1536.f, (_Float16)1536.f};
     h2_t x[2] = {pair(c.x), pair(c.y)};
@@ -271,7 +271,8 @@ extern "C" int dance_kv_compact(const DanceKvCache* from, const DanceKvCache* to
                                 uint32_t seqs, uint32_t width, const int32_t* keep, uint32_t keep_heads, uint32_t keep_width,
                                 const int32_t* counts, const int32_t* into_table, uint32_t into_width, void* stream) {
   using namespace dance::kv;
-  const DanceKvBatch source{table, lengths, nullptr, seqs, seqs, width, 1, 0}, target{into_table, counts, nullptr, seqs, seqs, into_width, 1, 0};
+  const DanceKvBatch source{table, lengths, nullptr, seqs, seqs, width, 1, 0};
+  const DanceKvBatch target{into_table, counts, nullptr, seqs, seqs, into_width, 1, 0};
   const char* why = check_common(from, &source);
   if (!why) why = check_common(to, &target);
   if (!why && (from->kv_heads != to->kv_heads || from->dim != to->dim || from->block_tokens != to->block_tokens))
@@ -284,7 +285,8 @@ extern "C" int dance_kv_compact(const DanceKvCache* from, const DanceKvCache* to
   // places that the lists can fill
   const uint32_t most = (keep_width - 1) / from->block_tokens + 1, places = most < into_width ? most : into_width;
   const uint64_t grid = (uint64_t)seqs * places * from->kv_heads;
-  if (grid > 0xFFFFFFFFull / 256) KV_ERR("dance_kv_compact", "batch is too large for one launch");
+  if (grid * 64 * compact_waves(from->dim, from->block_tokens) > 0xFFFFFFFFull)
+    KV_ERR("dance_kv_compact", "batch is too large for one launch");
   const Compact a{cache_args(from), cache_args(to), table, lengths, keep, counts, into_table,
                   width, keep_heads, keep_width, into_width, places};
   with_kind(from->dim, DANCE_KV_F16, [&](auto d, auto) {

@@ -367,7 +367,8 @@ def join(parts, lses, rows=None, *, out=None, return_lse=False):
     heads, dim] of one type, and the logarithms of their sums, [tokens, heads]
     float32, as return_lse gives them. Rows whose logarithm is -inf count for
     nothing. rows: for each part None, or [joined tokens] int32 with the part's row
-    for each joined one, and anything outside the part where it has none."""
+    for each joined one, and anything outside the part where it has none. out must not
+    overlap a part."""
     count = len(parts)
     if not 1 <= count <= 8 or len(lses) != count or (rows is not None and len(rows) != count):
         raise ValueError("1 to 8 parts, and as many lses and rows")
@@ -501,7 +502,8 @@ def compact(cache, keep, counts, table, lengths, into_table, into=None):
     """Writes chosen tokens densely into other blocks: token i < counts[b] of head h is
     the one at position keep[b, h, i] of sequence b (keep [sequences, kv_heads or 1,
     n] int32), and goes to the blocks of into_table [sequences, blocks] int32, of the cache `into` if
-    given. Blocks get the scales that append would give them. No block may be read and written."""
+    given. Blocks get the scales that append would give them. No block may be read and written, or named twice in
+    into_table."""
     into = cache if into is None else into
     _alike(cache, into)
     shape = table.shape

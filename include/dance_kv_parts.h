@@ -37,8 +37,9 @@ typedef struct DanceKvPart {
  * l_i a row's logarithms, out = sum_i exp(l_i - l) o_i and lse (may be null) l =
  * log sum_i exp(l_i), in float32 and rounded once. A part whose l_i is -infinity counts
  * for nothing, whatever its row holds; where all are, the row is zeros and
- * -infinity. 1 to 8 parts, all of `dtype`; a part without `rows` has `tokens`
- * rows; out is tokens x heads x dim of dtype and lse tokens x heads, packed. */
+ * -infinity; a NaN among them makes the row NaN. 1 to 8 parts, all of `dtype`; a part
+ * without `rows` has `tokens` rows; out is tokens x heads x dim of dtype and lse
+ * tokens x heads, packed, and neither overlaps a part. */
 int dance_kv_join(const DanceKvPart *parts, uint32_t count, uint32_t tokens, uint32_t heads, uint32_t dim, int dtype,
                   void *out, float *lse, void *stream);
 

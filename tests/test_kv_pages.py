@@ -688,10 +688,12 @@ def test_entries_refuse_before_any_device_work(capfd):
         args = [c, c, p, p, 2, 3, p, 2, 5, p, p, 3, None]
         args[i] = x
         calls.append((L.dance_kv_compact, args))
+    wide = fake(dim=256, block_tokens=128)[0]  # 512 threads a block: 2^33 in all
+    calls.append((L.dance_kv_compact, [wide, wide, p, p, 1 << 23, 3, p, 2, 128, p, p, 3, None]))
     for i, (fn, args) in enumerate(calls):
         capfd.readouterr()
         assert fn(*args) == -1, (i, fn.__name__, args)
-        assert fn.__name__ in capfd.readouterr().err
+        assert fn.__name__ in capfd.readouterr().err, (i, fn.__name__, args)
     assert L.dance_kv_copy(c, c, 1, None, None, 0, None) == 0  # no pairs: nothing to do
     assert L.dance_kv_release(ok, p, p, 2, 3, None, None, None) == 0
 
