@@ -24,15 +24,16 @@ struct Part {
   int64_t token_stride, head_stride;
   uint32_t tokens;
 };
+template <int P>
 struct Join {
-  Part part[kMostParts];
+  Part part[P];
   uint32_t heads, dim, pieces, rows, cover;  // pieces of eight dimensions in a row; rows x heads; rows that a workgroup covers
   uint16_t* __restrict__ out;
   float* __restrict__ lse;
 };
 
 template <int P, bool BF, bool VEC>
-__global__ __launch_bounds__(kThreads) void k_join_parts(Join a) {
+__global__ __launch_bounds__(kThreads) void k_join_parts(Join<P> a) {
   const uint32_t row = blockIdx.x * a.cover + threadIdx.x / a.pieces, piece = threadIdx.x % a.pieces;
   if (threadIdx.x >= a.cover * a.pieces || row >= a.rows) return;
   const uint32_t token = row / a.heads, head = row % a.heads;
@@ -107,7 +108,7 @@ extern "C" int dance_kv_join(const DanceKvPart* parts, uint32_t count, uint32_t 
   if (!why && (uint64_t)tokens * heads > 0x7FFFFFFFull) why = "batch is too large for one launch";
   if (!why && tokens && (!out || !aligned(out, 2))) why = "out must be given, aligned to its elements";
   bool vec = dim % 8 == 0 && aligned(out, 16);
-  Join a{};
+  Join<kMostParts> a{};
   for (uint32_t i = 0; !why && i < count; ++i) {
     const DanceKvPart& p = parts[i];
     if (p.tokens > 0x7FFFFFFFull) why = "a part must have fewer than 2^31 rows";
@@ -126,8 +127,12 @@ extern "C" int dance_kv_join(const DanceKvPart* parts, uint32_t count, uint32_t 
   const uint32_t grid = (a.rows + a.cover - 1) / a.cover;
   if ((uint64_t)grid * kThreads > 0xFFFFFFFFull) KV_ERR("dance_kv_join", "batch is too large for one launch");
   auto go = [&](auto n, auto bf, auto v) {
-    hipLaunchKernelGGL((k_join_parts<decltype(n)::value, decltype(bf)::value, decltype(v)::value>), dim3(grid), dim3(kThreads), 0,
-                       static_cast<hipStream_t>(stream), a);
+    constexpr int P = decltype(n)::value;
+    Join<P> b;
+    for (int i = 0; i < P; ++i) b.part[i] = a.part[i];
+    b.heads = a.heads, b.dim = a.dim, b.pieces = a.pieces, b.rows = a.rows, b.cover = a.cover, b.out = a.out, b.lse = a.lse;
+    hipLaunchKernelGGL((k_join_parts<P, decltype(bf)::value, decltype(v)::value>), dim3(grid), dim3(kThreads), 0,
+                       static_cast<hipStream_t>(stream), b);
   };
   auto kind = [&](auto n) {
     if (dtype == DANCE_KV_BF16)

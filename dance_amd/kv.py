@@ -83,8 +83,11 @@ _PART, _PAGES = struct.Struct("@PqqPPQ"), struct.Struct("@PII")
 assert [_CACHE.size, _BATCH.size, _ROWS.size, _PART.size, _PAGES.size] == [
     C.sizeof(t) for t in (DanceKvCache, DanceKvBatch, DanceKvRows, DanceKvPart, DanceKvPages)]
 
-# torch's handle of the current stream, without the Stream object around it where torch has that
+# torch's handle of the current stream, without the Stream object around it where torch has that, and the
+# current device without the look at whether there is one
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_I32 = torch.int32
 _bound = None
 _fast = {}
 
@@ -193,7 +196,7 @@ class Pages:
 
 
 def _ints(name, t, shape, device):
-    if t.dtype != torch.int32:
+    if t.dtype != _I32:
         raise TypeError(f"{name} must be int32")
     if t.shape != shape:
         raise ValueError(f"{name} must have the shape {tuple(shape)}")
@@ -247,7 +250,7 @@ def _batch(cache, tokens, table, lengths, offsets, max_tokens, max_length):
 
 
 def _launch(name, index, *args):
-    if torch.cuda.current_device() != index:
+    if _device() != index:
         with torch.cuda.device(index):
             rc = _fast[name](*args, _stream(index))
     else:
@@ -409,7 +412,7 @@ def join(parts, lses, rows=None, *, out=None, return_lse=False):
         args.append(_PART.pack(x.data_ptr(), strides[0], strides[1], lse.data_ptr(), own, shape[0]))
     shape = (tokens, heads, dim)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = torch.empty_like(first, memory_format=torch.contiguous_format) if first.shape == shape else first.new_empty(shape)
     elif out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {dtype} tensor {shape} on the parts' device")
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
@@ -420,11 +423,11 @@ def join(parts, lses, rows=None, *, out=None, return_lse=False):
 
 
 def _table(pages, table, lengths):
-    shape = table.shape
+    shape, device = table.shape, pages.device
     if len(shape) != 2 or 0 in shape:
         raise ValueError("table must be [sequences, blocks]")
-    _ints("table", table, shape, pages.device)
-    _ints("lengths", lengths, shape[:1], pages.device)
+    _ints("table", table, shape, device)
+    _ints("lengths", lengths, shape[:1], device)
     return shape
 
 
@@ -467,9 +470,10 @@ def release(pages, table, lengths, keep=None, start=None):
     keep tokens, and lengths follow; with start those of which all tokens stand before
     it, whose places become holes."""
     seqs, width = _table(pages, table, lengths)
-    for name, t in (("keep", keep), ("start", start)):
-        if t is not None:
-            _ints(name, t, (seqs,), pages.device)
+    if keep is not None:
+        _ints("keep", keep, (seqs,), pages.device)
+    if start is not None:
+        _ints("start", start, (seqs,), pages.device)
     _call("release", pages, table.data_ptr(), lengths.data_ptr(), seqs, width, _ptr(keep), _ptr(start))
 
 
