@@ -32,6 +32,21 @@ __device__ __forceinline__ float half_sum(float x) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+// The order of N loads from LDS and the products that they feed: four loads ahead, then one for each product. Left to
+// itself the compiler loads two and waits (two chunks of 2048 rows over 8000 tokens 526 us so, 486 four ahead; two of
+// 1024 over 4000 at 192 dimensions 276 and 262).
+template <int N, int GROUP>
+__device__ __forceinline__ void operands_ahead() {
+  constexpr int kProduct = 0x008, kLoad = 0x100, kFirst = 4;
+  __builtin_amdgcn_sched_group_barrier(kLoad, kFirst, GROUP);
+#pragma unroll
+  for (int i = 0; i < N - kFirst; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kProduct, 1, GROUP);
+    __builtin_amdgcn_sched_group_barrier(kLoad, 1, GROUP);
+  }
+  __builtin_amdgcn_sched_group_barrier(kProduct, kFirst, GROUP);
+}
+
 template <int D, bool BF, bool VEC, int W>
 __global__ __launch_bounds__(64 * W)
     __attribute__((amdgpu_waves_per_eu(chunk_occ(D), chunk_occ(D)))) void k_chunk(StepArgs a) {
@@ -227,6 +242,7 @@ __global__ __launch_bounds__(64 * W)
           const h8_t kf = *reinterpret_cast<const h8_t*>(sk[buf] + (u * 32u + n) * KST + c * 32 + hl * 16);
           sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[c], sc[u], 0, 0, 0);
         }
+      operands_ahead<2 * KS, 0>();
       const f4_t gk = *reinterpret_cast<const f4_t*>(sg[buf][0]), gl = *reinterpret_cast<const f4_t*>(sg[buf][1]),
                  gi = *reinterpret_cast<const f4_t*>(sg[buf][2]);
       const bool holes = fminf(fminf(gk.x, gk.y), fminf(gk.z, gk.w)) == -__builtin_inff();
@@ -286,6 +302,7 @@ __global__ __launch_bounds__(64 * W)
           const h8_t vf = *reinterpret_cast<const h8_t*>(sv[buf] + (d * 32u + n) * VST + j * 32 + hl * 16);
           acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[j], acc[d], 0, 0, 0);
         }
+      operands_ahead<4 * DT, 1>();
     }
     if constexpr (!kAhead) stage(tt);
   }
