@@ -12,7 +12,7 @@
 // operand wants: within 16 tokens 0-3, 8-11, 4-7, 12-15, a swap of words.
 //
 // Bound by the softmax's and the conversion's vector instructions and the matrix units in turn: two chunks of
-// 2048 tokens over 6,000 to 10,000, 8 kv heads of 4, 128 dimensions (491 GFLOP), 513 us, 957 TFLOP/s; a
+// 2048 tokens over 6,000 to 10,000, 8 kv heads of 4, 128 dimensions (491 GFLOP), 505 us, 972 TFLOP/s; a
 // large f16 product reaches 1370. Vector instructions are 54 %, matrix instructions 42 % of the time.
 #pragma once
 
