@@ -211,6 +211,37 @@ def test_pool_without_room():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("blocks", [30, 20000])  # one launch and two
+def test_reserve_of_nothing_and_of_what_is_there(blocks):
+    """Lengths that stay, go back or are no lengths; the same tensor for both; sequences that end on a block's last place."""
+    both = Both(Owners(blocks, 16, [[3, 4, -1], [5, -1, -1], [-1, -1, -1], [6, 7, 8], [-1, -1, -1]], [32, 16, 0, 41, 0]))
+    now, src, dst = both.reserve([32, 10, 0, -7, -2 ** 31])
+    assert now.tolist() == [32, 16, 0, 41, 0] and src.tolist() == [-1] * 5
+    kv.reserve(both.pages, both.table, both.lengths, both.lengths)
+    both.same()
+    now, _, _ = both.reserve([33, 17, 48, 48, 49])
+    assert now.tolist() == [33, 17, 48, 48, 0]
+    both.release(keep=both.m.lengths)
+    kv.release(both.pages, both.table, both.lengths, keep=both.lengths)
+    both.same()
+    both.release(start=[2 ** 31 - 1, 16, -2 ** 31, 31, 0])
+
+
+@pytest.mark.gpu
+def test_blocks_that_the_caller_keeps():
+    """One more owner for the blocks of a prompt: they outlive every sequence, and the partly filled one is always copied."""
+    both = Both(Owners(12, 16, [[2, 5, -1]], [20]))
+    for p in (2, 5):
+        both.m.refs[p] += 1
+        both.pages.refs[p] += 1
+    both.fork([0, 0, -1])
+    now, src, dst = both.reserve([21, 21, 0])
+    assert src.tolist() == [5, 5, -1] and dst.tolist() == [0, 1, -1] and now.tolist() == [21, 21, 0]
+    both.release(keep=[0, 0, 0])
+    assert both.m.refs == [0, 0, 1, 0, 0, 1] + [0] * 6
+
+
+@pytest.mark.gpu
 def test_places_reserved_ahead():
     """Room for more than is written: later calls find it, forks of it get their own."""
     both = Both(Owners(64, 16, [[9, -1, -1, -1, -1]], [3]))

@@ -250,6 +250,31 @@ def test_join_of_strided_parts_and_of_rows_that_count_for_nothing():
 
 
 @pytest.mark.gpu
+def test_join_of_logarithms_that_are_no_numbers():
+    x = torch.ones((4, 1, 8), dtype=F16, device="cuda")
+    a, b = (torch.tensor(v, device="cuda")[:, None] for v in ([math.nan, 1.0, math.nan, -math.inf], [1.0, math.nan, -math.inf, 2.0]))
+    got, lse = kv.join([x, 2 * x], [a, b], return_lse=True)
+    assert torch.isnan(got[:3]).all() and torch.isnan(lse[:3]).all() and (got[3] == 2).all() and float(lse[3]) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 90])
+def test_cross_attention_in_a_wide_table(rows):
+    """Blocks that a sequence has been given beyond its length count for nothing, with and without the longest length."""
+    rng = np.random.default_rng(36)
+    lens = [130, 64, 1]
+    cache, table = make(rng, 2, 128, 32, lens, spare=60)
+    wide = np.concatenate([table, np.setdiff1d(np.arange(cache.blocks), table)[:57].reshape(3, 19)], 1).astype(np.int32)
+    wide = np.where((wide < 0) | (wide >= cache.blocks), wide[:, -1:], wide)
+    off = offsets_of([rows] * 3)
+    q = torch.from_numpy(rng.normal(size=(off[-1], 4, 128))).to(BF16).cuda()
+    for longest in (None, 130):
+        got, lse = kv.cross_attention(cache, q, dev(wide), dev(np.int32(lens)), dev(off), max_tokens=rows, max_length=longest,
+                                      return_lse=True)
+        check_cross(Model(cache), got, lse, q, table, lens, off, 128 ** -0.5)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", [F16, BF16])
 def test_shared_prefix_and_own_tokens_equal_the_whole(dt):
     """Sequences of two groups that share their group's prompt: the prompt's blocks are read once for a group's rows, each
