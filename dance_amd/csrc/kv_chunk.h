@@ -12,7 +12,7 @@
 // operand wants: within 16 tokens 0-3, 8-11, 4-7, 12-15, a swap of words.
 //
 // Bound by the softmax's and the conversion's vector instructions and the matrix units in turn: two chunks of
-// 2048 tokens over 6,000 to 10,000, 8 kv heads of 4, 128 dimensions (491 GFLOP), 505 us, 972 TFLOP/s; a
+// 2048 tokens over 6,000 to 10,000, 8 kv heads of 4, 128 dimensions (491 GFLOP), 488 us, 1005 TFLOP/s; a
 // large f16 product reaches 1370. Vector instructions are 54 %, matrix instructions 42 % of the time.
 #pragma once
 
@@ -60,6 +60,9 @@ __global__ __launch_bounds__(64 * W)
   // The next tile's codes go to LDS ahead of a tile's products, which hide the conversion; with one wave a SIMD, behind
   // them (two chunks of 1024 rows over 4000 tokens: at 128 dimensions 5 % less, at 192 and 256 21 and 7 % more).
   constexpr bool kAhead = D <= 128;
+  // Blocks of a tile and more have addresses of their own (two chunks of 2048 rows over 8000 tokens 507 us without, 494
+  // with them; at 192 dimensions, where the registers then lie less well, 263 and 279 for two of 1024 over 4000).
+  constexpr bool kOneBlock = D != 192;
   __shared__ __attribute__((aligned(16))) char sk[2][64 * KST];
   __shared__ __attribute__((aligned(16))) char sv[2][D * VST];
   // of a tile's groups of 16 tokens: key scales (-infinity: a hole), log2 and inverses of the value scales
@@ -113,6 +116,19 @@ __global__ __launch_bounds__(64 * W)
   bool hole;
   auto load_codes = [&](uint32_t tt, int32_t raw) {
     const int32_t ph = entry(tt) < seen && (uint32_t)raw < a.c.blocks ? raw : -1;
+    if (kOneBlock && bsh >= 6) {  // the tile lies in one block: its place is the wave's, and a lane's offset in it stays
+      const uint32_t one = (uint32_t)max(__builtin_amdgcn_readfirstlane(ph), 0);
+      const size_t cell = (size_t)one * a.c.kvh + h;
+      const uint32_t slot = (tt * 64u) & (bs - 1u);
+      const int8_t* const k0 = a.c.k + ((cell << bsh) + slot) * D;
+      const int8_t* const v0 = a.c.v + ((cell * D) << bsh) + slot;
+#pragma unroll
+      for (int i = 0; i < CN; ++i) {
+        const uint32_t c = min(tid + i * 64 * W, kChunks - 1u);
+        kc[i] = *reinterpret_cast<const u4_t*>(k0 + c * 16u);
+        vc[i] = *reinterpret_cast<const u4_t*>(v0 + (((c >> 2) << bsh) + (c & 3u) * 16u));
+      }
+    } else {
 #pragma unroll
     for (int i = 0; i < CN; ++i) {
       const uint32_t c = min(tid + i * 64 * W, kChunks - 1u);
@@ -122,6 +138,7 @@ __global__ __launch_bounds__(64 * W)
       const size_t cell_k = (size_t)pk * a.c.kvh + h, cell_v = (size_t)pv * a.c.kvh + h;
       kc[i] = *reinterpret_cast<const u4_t*>(a.c.k + ((cell_k << bsh) + slot_k + (tok & 15u)) * D + off * 16);
       vc[i] = *reinterpret_cast<const u4_t*>(a.c.v + ((cell_v * D + (c >> 2)) << bsh) + slot_v);
+    }
     }
     if (tid < 4) {
       gs = *reinterpret_cast<const float2*>(a.c.scale + ((size_t)max(ph, 0) * a.c.kvh + h) * 2);
