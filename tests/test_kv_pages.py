@@ -438,6 +438,22 @@ def test_compact_of_far_apart_scales(scales):
         assert np.array_equal(numbers(cache.k[int(free[0, j]), 0]), codes_of(y.astype(np.float64), step))
 
 
+@pytest.mark.gpu
+def test_compact_of_the_least_code():
+    """-128, which append never writes, needs the next scale: 127 steps would not hold it."""
+    rng = np.random.default_rng(7)
+    cache, table = make(rng, 1, 64, 16, [16], spare=3)
+    p, free = int(table[0, 0]), int(np.setdiff1d(np.arange(cache.blocks), table)[0])
+    cache.k[p], cache.v[p], cache.scale[p] = -128, -128, 0.25
+    cache.k[p, :, 3], cache.v[p, :, :, 5] = 127, 1
+    keep = dev(np.arange(16, dtype=np.int32).reshape(1, 1, 16))
+    kv.compact(cache, keep, dev(np.int32([16])), dev(table), dev(np.int32([16])), dev(np.int32([[free]])))
+    assert (cache.scale[free] == 0.5).all()
+    k, v = cache.k[free, 0], cache.v[free, 0]
+    assert (k[3] == 64).all() and (k[4] == -64).all() and (v[:, 5] == 0).all() and (v[:, 4] == -64).all()  # halves to even
+    assert (cache.bound[free, 0, 0] == 64).all() and (cache.bound[free, 0, 1] == -64).all()
+
+
 # ------------------------------------------------------- as they are used together
 
 @pytest.mark.gpu
@@ -659,6 +675,20 @@ def test_refusals():
     kv.copy(cache, n[:0], n[:0])
     kv.release(pages, t, n)
     assert not pages.refs.any()
+
+
+@pytest.mark.parametrize("header,count", [("dance_kv_pages.h", 6), ("dance_kv_parts.h", 3)])
+def test_headers_are_c_and_their_entries_are_exported(header, count):
+    import re
+    import subprocess
+    import dance_amd as D
+    path = D.HERE + "/../include/" + header
+    for lang in ("c", "c++"):
+        subprocess.run(["gcc", "-x", lang, "-fsyntax-only", "-Wall", "-Wextra", "-Werror", path], check=True)
+    names = set(re.findall(r"\b(dance_kv_\w+)\(const", open(path).read()))
+    assert len(names) == count
+    out = subprocess.run(["nm", "-D", "--defined-only", D.LIB_PATH], capture_output=True, text=True).stdout
+    assert {n for n in names if f" T {n}\n" in out} == names
 
 
 def test_entries_refuse_before_any_device_work(capfd):
