@@ -79,7 +79,9 @@ int dance_kv_copy(const DanceKvCache *from, const DanceKvCache *to, uint32_t cac
  * i of into_table's row, into_width blocks of `to`. Its value x is the product of
  * its code and its scale in float32. A block's scale becomes the least that append
  * would choose for its values, the codes rint(x / scale), the bounds those of its
- * codes; behind the last token it holds zeros. A position that the sequence does not
+ * codes; behind the last token it holds zeros. As in append, a product that is not finite
+ * (a code times a scale above 2^121 may pass float32's range) counts for no scale: infinities
+ * take the code +-127, NaN the code 0. A position that the sequence does not
  * have, or that stands in a hole, gives a token of zeros. What falls beyond
  * into_table's row or into a hole of it is not written, counts beyond keep_width count as that. `to` has from's kv_heads, dim
  * and block_tokens; it may be `from`, but no block that is read may be written, and
