@@ -2,7 +2,8 @@
 // become the attention over all of it.
 //
 // With m the largest of a row's logarithms l_i, w_i = exp(l_i - m) and s = sum w_i, the row is sum w_i o_i / s
-// and its logarithm m + log s: float32, one rounding to the rows' type at the end. Every lane has
+// and its logarithm m + log s: float32, one rounding to the rows' type at the end. bfloat16 reaches float32's range, so that
+// a sum of eight rows would pass it: their weights are held in eighths, which changes no bit of normal numbers. Every lane has
 // eight dimensions of a row and forms the weights itself, so that nothing is exchanged. Bound by bytes: 8192 rows of 32
 // heads of 128, one part whole and two of half the rows (204 MB), 40 us, 5.1 TB/s, a large copy's rate; 64 rows of two
 // parts 3.6 us, a launch and three loads in turn.
@@ -47,14 +48,16 @@ __global__ __launch_bounds__(kThreads) void k_join_parts(Join<P> a) {
     l[p] = at[p] < x.tokens ? x.lse[(size_t)at[p] * a.heads + head] : -__builtin_inff();
     m = l[p] > m || l[p] != l[p] ? l[p] : m;
   }
+  constexpr float kUnit = BF ? 0.125f : 1.f;
   float w[P], sum = 0.f;
 #pragma unroll
   for (int p = 0; p < P; ++p) {
-    w[p] = l[p] == -__builtin_inff() ? 0.f : expf(l[p] - m);
-    sum += w[p];
+    const float x = l[p] == -__builtin_inff() ? 0.f : expf(l[p] - m);
+    sum += x;
+    w[p] = x * kUnit;
   }
   if (a.lse && piece == 0) a.lse[row] = m + logf(sum);  // -infinity where all parts are
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum * (1.f / kUnit);
   for (uint32_t d = piece * 8; d < a.dim; d += a.pieces * 8) {
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if constexpr (VEC) {
