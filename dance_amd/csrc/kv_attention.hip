@@ -52,9 +52,11 @@ constexpr uint32_t kStepWaves = 4;
 constexpr uint32_t kJoinWaves = 8;       // of k_join
 constexpr uint32_t kJoinCrossWaves = 4;  // of k_join_cross
 constexpr uint32_t kJoinFew = 16;        // splits that k_join_few takes, of rows that see their own part
-// Cross attention takes k_join below this many rows for each split: a workgroup a row costs 5.6 ns a row, a lane
-// that walks its splits 0.4 us a split. Measured, whole calls with k_join and k_join_few: 64 rows of 4 splits 17.4 and 17.7
-// us, of 16 22.1 and 27.6; 1024 of 8 19.4 and 17.7, of 16 23.1 and 25.1; 8192 of 24 233 and 223, of 64 308 and 325.
+// Cross attention joins by rows (k_join, k_join_cross) below this many rows for each split: a workgroup a row costs 5.6 ns
+// a row, a lane that walks its splits 0.4 us a split of few rows. Measured, calls of 16 heads of 64 in a graph, by rows and
+// with k_join_few: 64 rows of 4 splits 9.3 and 9.6 us, of 16 9.4 and 15.5; 1024 of 4 10.8 and 10.2, of 16 17.2 and 22.7; 8192
+// of 8 38.8 and 30.1, of 24 68.3 and 70.0. The limit is a straight line through a curve: 1024 rows of 8 splits (13.3 and
+// 14.2) and 8192 of 64 (151 and 166) take k_join_few, which is 7 and 9 % slower there.
 constexpr uint64_t kJoinRows = 128;
 constexpr uint64_t kJoinCrossRows = 256;  // from here on k_join_cross
 constexpr uint32_t kJoinThreads = 256;    // of k_join_few
@@ -599,7 +601,9 @@ struct Plan {
 // bytes; and the join. Fitted to 5,000 random shapes (64 to 256 dimensions, 1 to 20 kv heads of 1 to 16, 1 to 64 sequences,
 // 1 to 1500 rows, 20 to 60,000 tokens) with up to 30 plans each: on 800 others the chosen plans take 2.3 % more than the
 // best ones on average, those of the rules for rows that see their own part took 9 % more. 48 sequences of 1500 tokens, one row, 16
-// heads of 64: 27 us in one split, 31 in the two of those rules; 6 x 448 rows over 1500 tokens, 20 heads of 64: 46 and 54.
+// heads of 64: 28 us in one split, 31 in the two of those rules. Known to be too kind to k_step: the bytes count once, whatever
+// number of row tiles reads them, so that of the shapes with 17 to 128 rows a kv head one in ten takes k_step where k_chunk is
+// better, by 11 % on average and up to 62 (20 sequences of 8 rows, 2 kv heads of 8, 64 dimensions, over 55,000 tokens).
 struct Rates {
   double begin;
   double chain[5], tile[2][5];  // of each dimension; tile: of four waves, of eight
@@ -609,7 +613,7 @@ constexpr Rates kStepRates{
     5.9, {1.1, 1.2, 1.4, 1.6, 1.2}, {{0.67, 0.93, 1.4, 1.8, 1.8}, {0.61, 0.97, 1.3, 1.6, 1.7}}, {1.3, 1.7}, 6.4};
 constexpr Rates kChunkRates{
     8.7, {1.0, 1.4, 1.4, 0.0, 0.0}, {{0.59, 0.92, 1.0, 2.3, 3.1}, {0.52, 0.65, 0.73, 0.0, 0.0}}, {2.0, 3.2}, 120.0};
-constexpr double kJoinMb = 2.6, kJoinTime = 2.5, kJoinFewTime = 2.0, kJoinFewSplit = 0.24;
+constexpr double kJoinMb = 2.6, kJoinTime = 2.5, kJoinFewTime = 2.0, kJoinFewSplit = 0.24;  // beside the bytes
 constexpr uint32_t kCrossSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128};
 constexpr uint64_t kCrossStepRows = 1200, kCrossUnits = 4096;
 

@@ -12,8 +12,8 @@
 // operand wants: within 16 tokens 0-3, 8-11, 4-7, 12-15, a swap of words.
 //
 // Bound by the softmax's and the conversion's vector instructions and the matrix units in turn: two chunks of
-// 2048 tokens over 6,000 to 10,000, 8 kv heads of 4, 128 dimensions (491 GFLOP), 488 us, 1005 TFLOP/s; a
-// large f16 product reaches 1370. Vector instructions are 54 %, matrix instructions 42 % of the time.
+// 2048 tokens over 6,000 to 10,000, 8 kv heads of 4, 128 dimensions (491 GFLOP), 500 us, 980 TFLOP/s; a
+// large f16 product reaches 1370. Vector instructions are 55 %, matrix instructions 45 % of the time.
 #pragma once
 
 // Waves per SIMD, by registers. At 64 dimensions, where a tile has half the products for as much softmax, more waves
@@ -33,8 +33,8 @@ __device__ __forceinline__ float half_sum(float x) {
 }
 
 // The order of N loads from LDS and the products that they feed: four loads ahead, then one for each product. Left to
-// itself the compiler loads two and waits (two chunks of 2048 rows over 8000 tokens 526 us so, 486 four ahead; two of
-// 1024 over 4000 at 192 dimensions 276 and 262).
+// itself the compiler loads two and waits (two chunks of 2048 rows over 8000 tokens take 8 % less four ahead, two of 1024 over 4000 at 192
+// dimensions 5 %).
 template <int N, int GROUP>
 __device__ __forceinline__ void operands_ahead() {
   constexpr int kProduct = 0x008, kLoad = 0x100, kFirst = 4;
@@ -60,8 +60,8 @@ __global__ __launch_bounds__(64 * W)
   // The next tile's codes go to LDS ahead of a tile's products, which hide the conversion; with one wave a SIMD, behind
   // them (two chunks of 1024 rows over 4000 tokens: at 128 dimensions 5 % less, at 192 and 256 21 and 7 % more).
   constexpr bool kAhead = D <= 128;
-  // Blocks of a tile and more have addresses of their own (two chunks of 2048 rows over 8000 tokens 507 us without, 494
-  // with them; at 192 dimensions, where the registers then lie less well, 263 and 279 for two of 1024 over 4000).
+  // Blocks of a tile and more have addresses of their own (two chunks of 2048 rows over 8000 tokens take 3 % less so;
+  // at 192 dimensions, where the registers then lie less well, two of 1024 over 4000 take 6 % more).
   constexpr bool kOneBlock = D != 192;
   __shared__ __attribute__((aligned(16))) char sk[2][64 * KST];
   __shared__ __attribute__((aligned(16))) char sv[2][D * VST];

@@ -11,11 +11,12 @@
 // are bytes of different lines: lanes stand for neighbouring tokens, which mostly lie in the same lines, and leave as
 // words of four tokens that four lanes exchange by DPP.
 //
-// Measured: all tokens of 31 sequences of 15,000 to 21,000 copied (96 dimensions), 46 us, 4.9 TB/s, a large copy's
-// rate. Half of 16 sequences of 4,000 to 24,000 (8 heads of 128), other tokens for each head, 96 us: 290 MB that count,
-// 371 that move, since a line of values comes whole; 3.9 TB/s, and the units that form the byte loads' addresses are
-// busy for two thirds of the time. Every fiftieth token of 262,144: 49 us, 202 MB of lines (4.1 TB/s).
-// Lines read whole and bytes taken out of LDS: 90 us for half of the tokens, but 61 for all of the 31 sequences.
+// Measured: all tokens of 31 sequences of 15,000 to 21,000 (one head of 96 dimensions), 57 us, 3.9 TB/s; 44 us where
+// the cache behind the L2s holds them. Half of 16 sequences of 4,000 to 24,000 (8 heads of 128), other tokens for each
+// head, 96 us: 290 MB that count, 371 that move, since a line of values comes whole; 3.9 TB/s, and the units that form
+// the byte loads' addresses are busy for two thirds of the time. Every fiftieth token of 262,144: 51 us, 202 MB of lines
+// (4.0 TB/s). Lines read whole and bytes taken out of LDS: 6 % less for half of the tokens, a third more for all of the
+// 31 sequences.
 //
 // Between powers of two the arithmetic is f16's, two codes an instruction: a code is exact there, and c * ratio +
 // 1536 has the unit 1, so that one fma rounds it as the definition does and leaves the code in the low byte.

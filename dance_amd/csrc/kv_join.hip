@@ -5,8 +5,8 @@
 // and its logarithm m + log s: float32, one rounding to the rows' type at the end. bfloat16 reaches float32's range, so that
 // a sum of eight rows would pass it: their weights are held in eighths, which changes no bit of normal numbers. Every lane has
 // eight dimensions of a row and forms the weights itself, so that nothing is exchanged. Bound by bytes: 8192 rows of 32
-// heads of 128, one part whole and two of half the rows (204 MB), 40 us, 5.1 TB/s, a large copy's rate; 64 rows of two
-// parts 3.6 us, a launch and three loads in turn.
+// heads of 128, one part whole and two of half the rows (204 MB), 41 us, 5.0 TB/s, a large copy's rate; 64 rows of two
+// parts 3.5 us, a launch and three loads in turn.
 
 #include "../../include/dance_kv_parts.h"
 #include "kv_common.h"

@@ -3,10 +3,10 @@
 //
 // The first three are chains of dependent loads over little data (a table, a
 // count for each block), so they are bound by latency and by their launches; counts
-// change by integer atomics, whose order shows in no result. Measured: fork, reserve and
-// release of 32 sequences 3.0, 7.1 and 2.7 us, of 512 of up to 60,000 tokens over 173,005
-// blocks 7.0, 11.6 (two launches) and 3.0; a call costs the host 5 to 9 us. Copies run at a large copy's rate: 600 blocks
-// of 16 layers (2.6 GB moved) 488 us, 5.2 TB/s; 16 blocks of them 11 us.
+// change by integer atomics, whose order shows in no result. Measured, kernels alone: fork, reserve and
+// release of 32 sequences 3.2, 7.6 and 2.8 us, of 512 of up to 60,000 tokens over 173,005
+// blocks 7.1, 11.5 (two launches) and 3.0; a call costs the host 5 to 9 us. Copies run at a large copy's rate: 600 blocks
+// of 16 layers (2.6 GB moved) 502 us, 5.1 TB/s; 16 blocks of them 11 us.
 
 #include "../../include/dance_kv_pages.h"
 #include "kv_common.h"
@@ -48,7 +48,7 @@ constexpr uint32_t kTogether = 8;  // old rows that a workgroup looks at
 
 // Workgroups of old rows change the counts, by a row's children less one. A thread takes a place of several
 // rows: rows that lie together, as beams do, mostly share their first blocks, and what one of them loses there another
-// gains (128 users of 4 beams, 500 to 60,000 tokens in blocks of 32: 10.8 us with an atomic for each entry, 7.0
+// gains (128 users of 4 beams, 500 to 60,000 tokens in blocks of 32: 10.8 us with an atomic for each entry, 7.1
 // so). Workgroups of new rows copy them.
 __global__ __launch_bounds__(kThreads) void k_fork(Pages p, Table t, const int32_t* __restrict__ parents, uint32_t fresh,
                                                    uint32_t runs, uint32_t parts, uint32_t olds, int32_t* __restrict__ table,
